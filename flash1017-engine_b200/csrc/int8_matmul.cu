@@ -1,0 +1,551 @@
+// int8_matmul.cu -- products of dynamically quantised activations with int8
+// weights (W8A8): one scale per token, one per output channel, for one matrix
+// or for the rows of several experts.  The reference's integer matrices are
+// row-scaled int8 with f32 activations (HA:22-76); here both sides are int8.
+//
+//   s[r]      = fl32(max_c |x[r, c]| / 127),  q[r, c] = rne(fl32(x[r, c] / s[r]))
+//   acc[r, n] = sum_k q[r, k] w[g, n, k]                (exact, int32)
+//   out[r, n] = acc * s[r] * sw[g, n] + bias[g, n],  g the group of row r
+//
+// quant_kernel reads a row once into registers (DRAM-bound).  gemm_kernel runs
+// tcgen05.mma kind::i8 with the weights as the A operand: M = 128 channels, N =
+// up to 256 tokens, so that a decode step of one token fills the same 128 lanes
+// as a prefill and streams the weights at full width; accumulators in TMEM,
+// both operands staged by TMA (K-major rows of 128 bytes, 128-byte swizzle).
+#include <cuda.h>
+
+#include <algorithm>
+
+#include "ffn_internal.h"
+#include "rowops.cuh"
+#include "tcgen05.cuh"
+
+namespace ffn {
+namespace i8 {
+
+// ---------------------------------------------------------------- quantise
+struct QuantArgs {
+  const void *x;
+  size_t ld_x, ld_c;
+  int8_t *codes;
+  float *scales;
+  const int32_t *n_rows;  // DEVICE count of rows in use, or NULL
+  int rows;
+  uint32_t cols, n_vec;
+};
+
+// The framework's gated activation (flash1017.rs:7539) of gate g and up u.
+__device__ __forceinline__ float swiglu10(float g, float u) {
+  return fminf(g / (1.0f + expf(-g)), 10.0f) * fminf(fmaxf(u, -10.0f), 10.0f);
+}
+
+template <typename T, int VEC, int NV, bool WARP, bool SWIGLU>
+__global__ void __launch_bounds__(WARP ? 256 : 1024) quant_kernel(const QuantArgs a) {
+  __shared__ float s_red[32];
+  pdl_enter();
+  const uint32_t l = WARP ? threadIdx.x & 31 : threadIdx.x, L = WARP ? 32 : blockDim.x;
+  const long long row = WARP ? (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+  if (row >= a.rows || (a.n_rows && row >= __ldg(a.n_rows))) return;
+  const T *xr = (const T *)a.x + (size_t)row * a.ld_x;
+  Raw<T, VEC> rx[NV], ru[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t v = l + i * L;
+    if (v < a.n_vec) {
+      rx[i] = load_raw<T, VEC>(xr, v);
+      if (SWIGLU) ru[i] = load_raw<T, VEC>(xr + a.cols, v);
+    }
+  }
+  float f[NV][VEC];
+  float amax = 0.f;
+  bool fin = true;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t v = l + i * L;
+    if (v < a.n_vec) {
+      unpack<T, VEC>(rx[i], f[i]);
+      if (SWIGLU) {
+        float u[VEC];
+        unpack<T, VEC>(ru[i], u);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          fin = fin && isfinite(f[i][j]) && isfinite(u[j]);
+          f[i][j] = swiglu10(f[i][j], u[j]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        fin = fin && isfinite(f[i][j]);
+        amax = fmaxf(amax, fabsf(f[i][j]));
+      }
+    }
+  }
+  amax = warp_max(fin ? amax : INFINITY);
+  if (!WARP) {
+    const int lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+    if (lane == 0) s_red[threadIdx.x >> 5] = amax;
+    __syncthreads();
+    amax = warp_max(lane < nw ? s_red[lane] : 0.f);
+  }
+  const float sc = int8_scale(amax);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t v = l + i * L;
+    if (v < a.n_vec) store_codes<VEC>(a.codes + (size_t)row * a.ld_c + (size_t)v * VEC, f[i], sc);
+  }
+  if (l == 0) a.scales[row] = sc;
+}
+
+// ----------------------------------------------------------------- product
+constexpr int kThreads = 192;       // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
+constexpr int kM = 128;             // channels a tile
+constexpr int kKB = 128;            // K bytes (= values) a stage
+constexpr int kABytes = kM * kKB;
+constexpr int kMaxStages = 12;
+constexpr int kSmemMax = 224 * 1024;
+
+struct GemmArgs {
+  const int32_t *offsets;  // DEVICE [groups + 1] or NULL (one group of all rows)
+  const float *xs, *ws, *bias;
+  void *out;
+  size_t ld_out;
+  int rows, n, kt, groups;
+  int nt;      // tokens a tile, at most (16 .. 256)
+  int bx;      // rows of one token box
+  int stages;
+  int cs;      // CTAs of the cluster, each a part of K
+};
+
+__device__ __forceinline__ uint32_t idesc_i8(int M, int N) {  // s32 += s8 * s8, both K-major
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}\n"
+               ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc), "r"(0), "r"(0), "r"(0), "r"(0));
+}
+__device__ __forceinline__ void tma_2d(void *dst, const CUtensorMap *m, int x, int y, uint64_t *bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+               ::"r"(tc::sa(dst)), "l"(m), "r"(x), "r"(y), "r"(tc::sa(bar)) : "memory");
+}
+__device__ __forceinline__ void tma_prefetch_l2(const CUtensorMap *m, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(m), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ uint32_t ctarank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void st_peer(const void *p, uint32_t rank, int v) {
+  uint32_t b;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(tc::sa(p)), "r"(rank));
+  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(b), "r"(v) : "memory");
+}
+
+// One tile: 128 channels of group g from channel c0, tokens [r0, r0 + nn).
+struct Tile {
+  int g, c0, r0, nn;
+};
+// s_pre[g]: token chunks of the groups before g.  Tiles run over the groups,
+// inside a group over the channel blocks, inside a block over its token chunks,
+// so CTAs that run together share the weights' block.
+__device__ __forceinline__ Tile tile_of(int t, const GemmArgs &a, const int *s_pre, const int *s_off, int ct) {
+  int lo = 0, hi = a.groups;  // the last g with s_pre[g] * ct <= t
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if ((long long)s_pre[mid] * ct <= t) lo = mid; else hi = mid;
+  }
+  // skip empty groups: s_pre is equal there, the search ends on the last of them
+  const int chunks = s_pre[lo + 1] - s_pre[lo], rel = t - s_pre[lo] * ct;
+  const int first = s_off[2 * lo], n = s_off[2 * lo + 1];
+  const int per = ((n + chunks - 1) / chunks + 15) & ~15;
+  const int j = rel % chunks;
+  Tile o;
+  o.g = lo;
+  o.c0 = rel / chunks * kM;
+  o.r0 = first + j * per;
+  o.nn = max(0, min(per, n - j * per));
+  return o;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, const __grid_constant__ CUtensorMap mw,
+                                                           const __grid_constant__ CUtensorMap mx) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], mma_done;
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_err, s_sum[kThreads / 32];
+  uint8_t *smem = smem_raw + ((1024 - (tc::sa(smem_raw) & 1023)) & 1023);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int stage_bytes = kABytes + a.nt * kKB;
+  int *red = reinterpret_cast<int *>(smem + a.stages * stage_bytes);     // cs > 1: [cs][nt][128 / cs]
+  int *s_off = red + (a.cs > 1 ? kM * a.nt : 0);                          // [groups][first, count]
+  int *s_pre = s_off + 2 * a.groups;                                      // [groups + 1]
+  // two accumulators; one where a cluster has a single tile.  At most 64 columns
+  // then, so that every cluster CTA an SM can hold gets its own: clusters that
+  // waited for each other's TMEM on two SMs would wait for good.
+  const int acc_cols = a.nt, tmem_cols = a.cs > 1 ? max(32, acc_cols) : 2 * acc_cols;
+  const uint32_t rank = a.cs > 1 ? ctarank() : 0;
+  const int ct = (a.n + kM - 1) / kM;
+
+  if (tid == 0) {
+    s_err = 0;
+    for (int s = 0; s < a.stages; ++s) { tc::bar_init(&full[s], 1); tc::bar_init(&empty[s], 1); }
+    for (int b = 0; b < 2; ++b) { tc::bar_init(&acc_full[b], 1); tc::bar_init(&acc_empty[b], 4); }
+    tc::bar_init(&mma_done, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mw) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mx) : "memory");
+  }
+  if (warp == 1) tc::alloc(&s_tmem, tmem_cols);
+  const int k_lo = a.kt * (int)rank / a.cs, k_hi = a.kt * ((int)rank + 1) / a.cs;
+  const int tile0 = (int)(blockIdx.x / a.cs), tile_step = (int)(gridDim.x / a.cs);
+  if (!a.offsets && warp == 0 && lane < min(a.stages, k_hi - k_lo) ) {
+    // one group: this CTA's first weights are known before the previous kernel
+    // has finished; bring them into L2 (a hint, nothing is read from it yet)
+    const int chunks = (a.rows + a.nt - 1) / a.nt;
+    if (tile0 < chunks * ct) tma_prefetch_l2(&mw, (k_lo + lane) * kKB, tile0 / chunks * kM);
+  }
+  pdl_enter();
+
+  // token chunks of each group
+  if (a.offsets) {
+    const int per = (a.groups + kThreads - 1) / kThreads, g0 = min(tid * per, a.groups), g1 = min(g0 + per, a.groups);
+    int sum = 0;
+    for (int g = g0; g < g1; ++g) {
+      // bounds from the GPU: kept inside the rows whatever they hold
+      const int lo = min(max(__ldg(a.offsets + g), 0), a.rows), hi = min(max(__ldg(a.offsets + g + 1), lo), a.rows);
+      s_off[2 * g] = lo;
+      s_off[2 * g + 1] = hi - lo;
+      s_pre[g] = sum;
+      sum += (hi - lo + a.nt - 1) / a.nt;
+    }
+    int inc = sum;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    if (lane == 31) s_sum[warp] = inc;
+    __syncthreads();
+    int base = inc - sum;
+    for (int w = 0; w < warp; ++w) base += s_sum[w];
+    for (int g = g0; g < g1; ++g) s_pre[g] += base;
+    if (tid == kThreads - 1) s_pre[a.groups] = base + sum;
+  } else if (tid == 0) {
+    s_off[0] = 0;
+    s_off[1] = a.rows;
+    s_pre[0] = 0;
+    s_pre[1] = (a.rows + a.nt - 1) / a.nt;
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  if (a.cs > 1) cluster_sync();  // the peers' shared memory is there
+  const uint32_t tmem = s_tmem;
+  const int n_tiles = s_pre[a.groups] * ct;
+
+  if (warp == 0) {
+    // -------------------------------------------------- TMA producer (one lane)
+    if (lane == 0) {
+      int it = 0;
+      bool live = true;
+      for (int t = tile0; t < n_tiles && live; t += tile_step) {
+        const Tile o = tile_of(t, a, s_pre, s_off, ct);
+        const int boxes = (o.nn + a.bx - 1) / a.bx;
+        const uint32_t bytes = kABytes + boxes * a.bx * kKB;
+        for (int k = k_lo; k < k_hi; ++k, ++it) {
+          const int s = it % a.stages;
+          if (!tc::bar_wait(&empty[s], ((it / a.stages) & 1) ^ 1, &s_err)) { live = false; break; }
+          uint8_t *st = smem + s * stage_bytes;
+          tc::bar_arrive_tx(&full[s], bytes);
+          tma_2d(st, &mw, k * kKB, o.g * a.n + o.c0, &full[s]);
+          for (int b = 0; b < boxes; ++b)
+            tma_2d(st + kABytes + b * a.bx * kKB, &mx, k * kKB, o.r0 + b * a.bx, &full[s]);
+        }
+      }
+      // every copy has landed before the CTA leaves
+      for (int s = 0; s < min(a.stages, it); ++s) {
+        const int last = (it - 1 - s) / a.stages;  // the last use of stage s
+        tc::bar_wait_drain(&full[s], last & 1);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // -------------------------------------------------- MMA issuer (one lane)
+    if (lane == 0) {
+      int it = 0, n = 0;
+      bool live = true;
+      for (int t = tile0; t < n_tiles && live; t += tile_step, ++n) {
+        const Tile o = tile_of(t, a, s_pre, s_off, ct);
+        const uint32_t id = idesc_i8(kM, max(16, (o.nn + 15) & ~15));
+        const int b = n & 1;
+        if (!tc::bar_wait(&acc_empty[b], ((n >> 1) & 1) ^ 1, &s_err)) break;
+        tc::fence_after();
+        for (int k = k_lo; k < k_hi; ++k, ++it) {
+          const int s = it % a.stages;
+          if (!tc::bar_wait(&full[s], (it / a.stages) & 1, &s_err)) { live = false; break; }
+          tc::fence_after();
+          const uint32_t sa = tc::sa(smem + s * stage_bytes);
+#pragma unroll
+          for (int j = 0; j < kKB / 32; ++j)
+            mma_i8(tmem + b * acc_cols, tc::desc_sw128(sa + 32 * j), tc::desc_sw128(sa + kABytes + 32 * j), id,
+                   (k > k_lo || j > 0) ? 1u : 0u);
+          tc::commit(&empty[s]);
+        }
+        if (!live) break;
+        tc::commit(&acc_full[b]);
+      }
+      tc::commit(&mma_done);  // every MMA has completed before TMEM is freed
+      tc::bar_wait_drain(&mma_done, 0);
+    }
+    __syncwarp();
+  } else {
+    // -------------------------------------------------- epilogue (4 warps)
+    const int quarter = warp & 3, cl = quarter * 32 + lane;
+    int n = 0;
+    for (int t = tile0; t < n_tiles; t += tile_step, ++n) {
+      const Tile o = tile_of(t, a, s_pre, s_off, ct);
+      const int b = n & 1;
+      const bool ok = __all_sync(0xffffffffu, tc::bar_wait(&acc_full[b], (n >> 1) & 1, &s_err));
+      tc::fence_after();
+      const uint32_t tl = tmem + b * acc_cols + ((uint32_t)(32 * quarter) << 16);
+      if (a.cs > 1) {
+        // this CTA's part of K: lane cl's sums go to the CTA that owns the channel
+        const int own = kM / a.cs, dst = cl / own;
+        for (int c = 0; ok && c < o.nn; c += 16) {
+          uint32_t v[16];
+          tc::ld16(tl + c, v);
+          tc::wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (c + j < o.nn) st_peer(red + ((int)rank * a.nt + c + j) * own + cl % own, dst, (int)v[j]);
+        }
+        break;  // one tile a cluster; the sums are added up below
+      }
+      const int ch = o.c0 + cl;
+      const bool on = ch < a.n;
+      const float sw = on ? __ldg(a.ws + (size_t)o.g * a.n + ch) : 0.f;
+      const float bias = on && a.bias ? __ldg(a.bias + (size_t)o.g * a.n + ch) : 0.f;
+      T *out = reinterpret_cast<T *>(a.out) + (size_t)o.r0 * a.ld_out + ch;
+      for (int c = 0; c < o.nn; c += 16) {
+        uint32_t v[16];
+        if (ok) {
+          tc::ld16(tl + c, v);
+          tc::wait_ld();
+        }
+        const float sx = c + (lane & 15) < o.nn ? __ldg(a.xs + o.r0 + c + (lane & 15)) : 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float s = __shfl_sync(0xffffffffu, sx, j);
+          // a wait that ran out leaves NaN behind
+          const float f = ok ? (float)(int)v[j] * s * sw + bias : __int_as_float(0x7fffffff);
+          if (on && c + j < o.nn) out[(size_t)(c + j) * a.ld_out] = ToF32<T>::put(f);
+        }
+      }
+      tc::fence_before();
+      __syncwarp();
+      if (lane == 0) tc::bar_arrive(&acc_empty[b]);
+    }
+  }
+  if (a.cs > 1) {
+    __syncthreads();
+    if (s_err && tid < a.cs) st_peer(&s_err, tid, 1);  // all CTAs of the cluster learn of it
+    __syncwarp();
+    cluster_sync();
+    if (tile0 < n_tiles) {
+      const Tile o = tile_of(tile0, a, s_pre, s_off, ct);
+      const int own = kM / a.cs;
+      for (int i = tid; i < o.nn * own; i += kThreads) {
+        const int r = i / own, c = i % own, ch = o.c0 + (int)rank * own + c;
+        if (ch >= a.n) continue;
+        int acc = 0;
+        for (int q = 0; q < a.cs; ++q) acc += red[(q * a.nt + r) * own + c];
+        float f = (float)acc * __ldg(a.xs + o.r0 + r) * __ldg(a.ws + (size_t)o.g * a.n + ch);
+        if (a.bias) f += __ldg(a.bias + (size_t)o.g * a.n + ch);
+        if (s_err) f = __int_as_float(0x7fffffff);
+        reinterpret_cast<T *>(a.out)[(size_t)(o.r0 + r) * a.ld_out + ch] = ToF32<T>::put(f);
+      }
+    }
+  }
+  tc::fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc::fence_after();
+    tc::dealloc(tmem, tmem_cols);
+  }
+}
+
+// ------------------------------------------------------------------ launch
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                              const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static const EncodeFn fn = [] {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return (EncodeFn)p;
+  }();
+  return fn;
+}
+// rows x k bytes at p, ld bytes apart; boxes of 128 bytes x box_rows; bytes
+// past k and rows past the end read as 0
+int encode(CUtensorMap *m, const void *p, size_t rows, size_t k, size_t ld, int box_rows) {
+  const EncodeFn fn = encode_fn();
+  if (!fn) return fail(FFN_B200_ECUDA, "int8_matmul: the driver has no cuTensorMapEncodeTiled");
+  const cuuint64_t dim[2] = {k, rows}, stride[1] = {ld};
+  const cuuint32_t box[2] = {(cuuint32_t)kKB, (cuuint32_t)box_rows}, es[2] = {1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(p), dim, stride, box, es,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(FFN_B200_EINVAL, "int8_matmul: tensor map refused (code " + std::to_string((int)r) + ")");
+  return 0;
+}
+
+template <typename T>
+int launch_gemm(const GemmArgs &a, int grid, size_t smem, const CUtensorMap &mw, const CUtensorMap &mx, int dev,
+                cudaStream_t st) {
+  static bool attr[64] = {false};
+  if (!attr[dev]) {
+    FFN_CUDA_TRY(cudaFuncSetAttribute(gemm_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax));
+    attr[dev] = true;
+  }
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = pdl_allowed() ? 1 : 0;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = a.cs;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = a.cs > 1 ? 2 : 1;
+  prof_begin(FFN_B200_K_INT8_GEMM, st);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_kernel<T>, a, mw, mx);
+  prof_end(FFN_B200_K_INT8_GEMM, st);
+  note_launch();
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return cuda_fail(e, "int8_matmul");
+  }
+  return 0;
+}
+
+template <typename T, int VEC, bool SWIGLU>
+int launch_quant(QuantArgs &a, cudaStream_t st) {
+  a.n_vec = a.cols / VEC;
+#define FFN_GO(NV, W, GRID, THREADS) \
+  FFN_LAUNCH_PDL(FFN_B200_K_INT8_QUANT, st, "quantize_int8", (quant_kernel<T, VEC, NV, W, SWIGLU>), GRID, THREADS, 0, a)
+  // short rows a warp each, longer ones a CTA of just enough threads
+  if constexpr (VEC > 1) {
+    if (a.n_vec <= 128) FFN_GO(4, true, (a.rows + 7) / 8, 256);
+    else if (a.n_vec <= 2048) FFN_GO(2, false, a.rows, (int)((a.n_vec + 63) / 64 * 32));
+    else FFN_GO(4, false, a.rows, (int)((a.n_vec + 127) / 128 * 32));
+  } else {
+    if (a.n_vec <= 512) FFN_GO(16, true, (a.rows + 7) / 8, 256);
+    else FFN_GO(16, false, a.rows, (int)((a.n_vec + 511) / 512 * 32));
+  }
+#undef FFN_GO
+  return 0;
+}
+template <typename T, int VEC>
+int launch_quant_act(QuantArgs &a, int act, cudaStream_t st) {
+  return act == FFN_B200_ACT_SWIGLU ? launch_quant<T, VEC, true>(a, st) : launch_quant<T, VEC, false>(a, st);
+}
+
+}  // namespace i8
+}  // namespace ffn
+
+using namespace ffn;
+
+extern "C" {
+
+int ffn_b200_quantize_int8(size_t rows, size_t cols, int32_t dtype, const void *x, size_t ld_x, int32_t act,
+                           const int32_t *n_rows, int8_t *codes, size_t ld_codes, float *scales, void *stream) {
+  using namespace ffn::i8;
+  if (!dtype_ok(dtype)) return fail(FFN_B200_EINVAL, "quantize_int8: unknown dtype");
+  if (act != FFN_B200_ACT_NONE && act != FFN_B200_ACT_SWIGLU) return fail(FFN_B200_EINVAL, "quantize_int8: unknown act");
+  if (cols == 0 || cols > 16384) return fail(FFN_B200_EUNSUP, "quantize_int8: cols must be in 1..16384");
+  if (rows > 0x7fffffffu) return fail(FFN_B200_EINVAL, "quantize_int8: too many rows");
+  if (rows == 0) return 0;
+  if (!x || !codes || !scales) return fail(FFN_B200_EINVAL, "quantize_int8: null pointer");
+  const size_t width = act == FFN_B200_ACT_SWIGLU ? 2 * cols : cols, es = dtype_bytes(dtype);
+  if (rows > 1 && (ld_x < width || ld_codes < cols)) return fail(FFN_B200_EINVAL, "quantize_int8: rows overlap");
+  if ((uintptr_t)x % es || (uintptr_t)scales % 4)
+    return fail(FFN_B200_EINVAL, "quantize_int8: rows and scales must be aligned to their type");
+  QuantArgs a{};
+  a.x = x, a.ld_x = ld_x, a.codes = codes, a.ld_c = ld_codes, a.scales = scales, a.n_rows = n_rows;
+  a.rows = (int)rows, a.cols = (uint32_t)cols;
+  const bool v16 = cols * es % 16 == 0 && rows16(x, ld_x, es) && (((uintptr_t)codes | ld_codes) & 7) == 0;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == FFN_B200_DT_F32) return v16 ? launch_quant_act<float, 4>(a, act, st) : launch_quant_act<float, 1>(a, act, st);
+  if (dtype == FFN_B200_DT_BF16)
+    return v16 ? launch_quant_act<__nv_bfloat16, 8>(a, act, st) : launch_quant_act<__nv_bfloat16, 1>(a, act, st);
+  return v16 ? launch_quant_act<__half, 8>(a, act, st) : launch_quant_act<__half, 1>(a, act, st);
+}
+
+int ffn_b200_int8_matmul(size_t rows, size_t n, size_t k, size_t n_groups, const int32_t *offsets, const int8_t *x,
+                         size_t ld_x, const float *x_scales, const int8_t *w, size_t ld_w, const float *w_scales,
+                         const float *bias, int32_t dtype, void *out, size_t ld_out, void *stream) {
+  using namespace ffn::i8;
+  if (!dtype_ok(dtype)) return fail(FFN_B200_EINVAL, "int8_matmul: unknown dtype");
+  if (n == 0 || k == 0 || k > 131072) return fail(FFN_B200_EUNSUP, "int8_matmul: n must be positive and k in 1..131072");
+  if (n_groups == 0 || n_groups > 4096) return fail(FFN_B200_EINVAL, "int8_matmul: n_groups must be in 1..4096");
+  if (n_groups > 1 && !offsets) return fail(FFN_B200_EINVAL, "int8_matmul: several groups need offsets");
+  if (rows > (1u << 30) || n > (1u << 30) / n_groups) return fail(FFN_B200_EINVAL, "int8_matmul: too many rows");
+  if (rows == 0) return 0;
+  if (!x || !x_scales || !w || !w_scales || !out) return fail(FFN_B200_EINVAL, "int8_matmul: null pointer");
+  if (((uintptr_t)x | (uintptr_t)w | ld_x | ld_w) % 16)
+    return fail(FFN_B200_EINVAL, "int8_matmul: x, w and their row strides must be multiples of 16 bytes");
+  if (ld_x < k || ld_w < k || (rows > 1 && ld_out < n)) return fail(FFN_B200_EINVAL, "int8_matmul: rows overlap");
+  if ((uintptr_t)out % dtype_bytes(dtype) || ((uintptr_t)x_scales | (uintptr_t)w_scales | (uintptr_t)bias) % 4)
+    return fail(FFN_B200_EINVAL, "int8_matmul: out and scales must be aligned to their type");
+  int dev = 0;
+  FFN_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return fail(FFN_B200_EUNSUP, "int8_matmul: device index >= 64");
+  const int sms = sm_count_of(dev);
+  GemmArgs a{};
+  a.offsets = offsets;
+  a.xs = x_scales, a.ws = w_scales, a.bias = bias;
+  a.out = out, a.ld_out = ld_out;
+  a.rows = (int)rows, a.n = (int)n, a.groups = (int)n_groups;
+  a.kt = (int)((k + kKB - 1) / kKB);
+  // tokens a tile: the smallest that holds an average group (a third on top for
+  // uneven ones)
+  const size_t avg = offsets ? (rows + n_groups - 1) / n_groups * 4 / 3 : rows;
+  a.nt = avg <= 16 ? 16 : avg <= 32 ? 32 : avg <= 64 ? 64 : avg <= 128 ? 128 : 256;
+  a.bx = std::min(a.nt, 64);
+  const long long ct = (long long)((n + kM - 1) / kM);
+  // tiles at most: each group may end in a partial chunk
+  const long long chunks = offsets ? std::min<long long>(rows, rows / a.nt + n_groups) : (rows + a.nt - 1) / a.nt;
+  const long long tiles = ct * chunks;
+  // (the kernel's tile numbers stay in 32 bits even where offsets are not ascending)
+  if ((double)(rows / a.nt + 1) * (double)n_groups * (double)ct > 2147483647.0) return fail(FFN_B200_EINVAL, "int8_matmul: too many tiles");
+  // few tiles: K split over a cluster
+  a.cs = 1;
+  if (a.nt <= 64)
+    while (a.cs < 8 && tiles * a.cs * 2 <= sms && a.kt >= 4 * a.cs) a.cs *= 2;
+  const size_t tail = (a.cs > 1 ? (size_t)kM * a.nt * 4 : 0) + (3 * n_groups + 1) * sizeof(int);
+  const size_t stage = (size_t)kABytes + (size_t)a.nt * kKB;
+  a.stages = (int)std::min<size_t>({(kSmemMax - 1024 - tail) / stage, (size_t)kMaxStages, (size_t)std::max(2, a.kt)});
+  if (a.stages < 2) return fail(FFN_B200_EUNSUP, "int8_matmul: too many groups for shared memory");
+  const size_t smem = 1024 + a.stages * stage + tail;
+  CUtensorMap mw, mx;
+  if (int rc = encode(&mw, w, n_groups * n, k, ld_w, kM)) return rc;
+  if (int rc = encode(&mx, x, rows, k, ld_x, a.bx)) return rc;
+  const int grid = a.cs > 1 ? (int)tiles * a.cs : (int)std::min<long long>(tiles, sms);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == FFN_B200_DT_F32) return launch_gemm<float>(a, grid, smem, mw, mx, dev, st);
+  if (dtype == FFN_B200_DT_BF16) return launch_gemm<__nv_bfloat16>(a, grid, smem, mw, mx, dev, st);
+  return launch_gemm<__half>(a, grid, smem, mw, mx, dev, st);
+}
+
+}  // extern "C"

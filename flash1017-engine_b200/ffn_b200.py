@@ -20,6 +20,9 @@ SCORE_REF, SCORE_SIGMOID = 0, 1
 ROUTER_EXACT, ROUTER_TENSOR = 0, 1
 PATH_AUTO, PATH_GEMV, PATH_GROUPED, PATH_FP4 = 0, 1, 2, 3
 GROUPED_MIN_PAIRS = 48
+DT_F32, DT_BF16, DT_F16 = 0, 1, 2
+ACT_NONE, ACT_SWIGLU = 0, 1
+GATE_NONE, GATE_CHANNEL, GATE_TOKEN = 0, 1, 2
 ERRORS = {0: "OK", -1: "EINVAL", -2: "ECUDA", -3: "ENOSPC", -4: "ENCCL", -5: "EUNSUP"}
 
 # Symbols the public headers declare (checked by the CPU test suite).
@@ -46,15 +49,19 @@ EXPORTS = [
     "ffn_b200_quantize_nvfp4x4", "ffn_b200_ep_moe_layer", "ffn_b200_set_host_cache_budget",
     "ffn_b200_topk", "ffn_b200_quantize_nvfp4_terms", "ffn_b200_fp4_pack_bytes",
     "ffn_b200_pack_nvfp4_expert",
+    "ffn_b200_quantize_int8", "ffn_b200_int8_matmul",
+    "ffn_b200_moe_sort", "ffn_b200_moe_permute", "ffn_b200_moe_combine", "ffn_b200_moe_combine_bwd",
+    "ffn_b200_block_norm", "ffn_b200_block_norm_bwd_ws_bytes", "ffn_b200_block_norm_bwd",
 ]
 
 # Kernel kinds of ffn_b200_profile_read (FFN_B200_K_*).
 K_XPREP, K_ROUTER, K_TOPK, K_GROUP, K_GATEUP_NVFP4, K_DOWN_NVFP4 = 0, 1, 2, 3, 4, 5
 K_GATEUP_TERNARY, K_DOWN_TERNARY, K_COREZ, K_COMBINE, K_MATVEC, K_OTHER = 6, 7, 8, 9, 10, 11
 K_GEMM_GATEUP, K_GEMM_DOWN, K_QUANT, K_FP4_GATEUP, K_FP4_DOWN = 12, 13, 14, 15, 16
+K_ROUTE, K_NORM, K_INT8_QUANT, K_INT8_GEMM = 17, 18, 19, 20
 K_NAMES = ["xprep", "router", "topk", "group", "gateup_nvfp4", "down_nvfp4", "gateup_ternary",
            "down_ternary", "corez", "combine", "matvec", "other", "gemm_gateup", "gemm_down",
-           "quant", "fp4_gateup", "fp4_down"]
+           "quant", "fp4_gateup", "fp4_down", "route", "norm", "int8_quant", "int8_gemm"]
 
 
 def build() -> str:
@@ -91,6 +98,13 @@ class MoeDesc(C.Structure):
                 ("expert_end", C.c_int32), ("has_nvfp4", C.c_int32),
                 ("has_ternary", C.c_int32), ("norm_w", C.c_void_p), ("norm_eps", C.c_float),
                 ("path", C.c_int32), ("has_mxfp4", C.c_int32), ("fp4_packed", C.c_int32)]
+
+
+class BlockNormDesc(C.Structure):
+    _fields_ = [("rows", C.c_size_t), ("cols", C.c_size_t), ("dtype", C.c_int32),
+                ("gate_kind", C.c_int32), ("post_w", C.c_void_p), ("gate", C.c_void_p),
+                ("pre_w", C.c_void_p), ("alpha", C.c_float), ("beta", C.c_float),
+                ("eps", C.c_float), ("reserved", C.c_uint32)]
 
 
 assert C.sizeof(Expert) == 264, C.sizeof(Expert)
@@ -183,6 +197,21 @@ def lib() -> C.CDLL:
         L.ffn_b200_ep_error.argtypes = [vp, C.POINTER(C.c_int)]
         L.ffn_b200_ep_destroy.argtypes = [vp]
         L.ffn_b200_profile_read.argtypes = [i32, C.POINTER(C.c_double), C.POINTER(C.c_uint64)]
+        L.ffn_b200_quantize_int8.argtypes = [sz, sz, C.c_int32, vp, sz, C.c_int32, vp, vp, sz, vp, vp]
+        L.ffn_b200_int8_matmul.argtypes = [sz, sz, sz, sz, vp, vp, sz, vp, vp, sz, vp, vp, C.c_int32,
+                                           vp, sz, vp]
+        L.ffn_b200_moe_sort.argtypes = [sz, sz, vp, C.c_int32, C.c_int32, vp, vp, vp, vp]
+        L.ffn_b200_moe_permute.argtypes = [sz, sz, sz, vp, sz, vp, sz, vp, sz, vp, vp, vp]
+        L.ffn_b200_moe_combine.argtypes = [sz, sz, sz, C.c_int32, vp, sz, sz, vp, vp, vp, sz, vp, sz,
+                                           vp]
+        L.ffn_b200_moe_combine_bwd.argtypes = [sz, sz, sz, C.c_int32, vp, sz, vp, sz, sz, vp, vp, vp,
+                                               sz, vp, vp]
+        pd = C.POINTER(BlockNormDesc)
+        L.ffn_b200_block_norm.argtypes = [pd, vp, sz, vp, sz, vp, sz, vp, sz, vp, sz, vp, vp]
+        L.ffn_b200_block_norm_bwd_ws_bytes.restype = sz
+        L.ffn_b200_block_norm_bwd_ws_bytes.argtypes = [pd]
+        L.ffn_b200_block_norm_bwd.argtypes = [pd, vp, sz, vp, sz, vp, sz, vp, sz, vp, sz, vp, sz, vp,
+                                              vp, vp, vp, sz, vp]
         L.ffn_b200_st_open.argtypes = [C.c_char_p, C.POINTER(vp)]
         L.ffn_b200_st_close.argtypes = [vp]
         L.ffn_b200_st_count.argtypes = [vp]
@@ -773,3 +802,455 @@ class MoeLayer:
                                        _ptr(out), _ptr(topk_idx), _ptr(topk_w), _ptr(ws),
                                        ws.numel(), _stream(stream)), "moe_layer")
         return out
+
+
+# ------------------------------------------------ activation rows of any type
+# The operators below take rows of f32, bf16 or f16: 2-d CUDA tensors whose rows
+# may be slices of wider ones.  Rows that are not contiguous inside are copied;
+# outputs are written in place.  `stream`: where the kernels run and what is
+# returned belongs to (default: the current stream of the tensors' device).
+# Temporaries come from torch's allocator, so calls on several streams and
+# captured graphs share none.  Nothing here takes part in autograd: the
+# gradients are calls of their own.
+_dts = None
+
+
+def _dtype(t):
+    global _dts
+    if _dts is None:
+        torch = _torch()
+        _dts = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
+    d = _dts.get(t.dtype)
+    if d is None:
+        raise FfnError(f"rows must be float32, bfloat16 or float16, not {t.dtype}")
+    return d
+
+
+def _elsewhere(t, stream):
+    """Whether a call on t has to switch device or stream first."""
+    if not t.is_cuda:
+        raise FfnError("expected CUDA tensors")
+    return stream is not None or t.device.index != _torch().cuda.current_device()
+
+
+def _on(t, stream):
+    torch = _torch()
+    if stream is None:
+        return torch.cuda.device(t.device)
+    if stream.device != t.device:
+        raise FfnError(f"the stream is on {stream.device}, the tensors on {t.device}")
+    return torch.cuda.stream(stream)
+
+
+def _raw(t):
+    """The current stream of t's device, as the library takes it."""
+    return _torch().cuda.current_stream(t.device).cuda_stream
+
+
+def _in(t, what, like, rows=None, cols=None, dtype=None):
+    """t as rows the library reads: 2-d, contiguous inside a row."""
+    if t.dim() != 2 or (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
+        raise FfnError(f"{what}: expected shape [{'rows' if rows is None else rows}, "
+                       f"{'cols' if cols is None else cols}], got {list(t.shape)}")
+    if t.device != like.device:
+        raise FfnError(f"{what} is on {t.device}, not on {like.device}")
+    if t.dtype != (like.dtype if dtype is None else dtype):
+        raise FfnError(f"{what}: expected {like.dtype if dtype is None else dtype}, got {t.dtype}")
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t
+
+
+def _out(t, what, like, rows, cols, dtype=None):
+    """t as rows the library writes, or new rows."""
+    if t is None:
+        return _torch().empty(rows, cols, dtype=like.dtype if dtype is None else dtype, device=like.device)
+    if _in(t, what, like, rows, cols, dtype) is not t:
+        raise FfnError(f"{what}: output rows must be contiguous and must not overlap")
+    return t
+
+
+def _vec(t, what, like, n, dtype=None):
+    """t as n contiguous values (float32 unless said otherwise)."""
+    dtype = _torch().float32 if dtype is None else dtype
+    if t.dtype != dtype or t.device != like.device or t.numel() != n or not t.is_contiguous():
+        raise FfnError(f"{what}: expected {n} contiguous {dtype} values on {like.device}, got "
+                       f"{list(t.shape)} {t.dtype} on {t.device}")
+    return t
+
+
+def _ld(t):
+    """Row stride in elements; that of a single row may be anything."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def quantize_int8(x, act=ACT_NONE, codes=None, scales=None, n_rows=None, stream=None):
+    """Rows x [rows, cols] (act ACT_SWIGLU: [rows, 2 cols], gate then up) ->
+    (codes int8 [rows, cols], scales f32 [rows]), one scale a row
+    (ffn_b200_quantize_int8).  New codes are a view of rows padded to 16 bytes,
+    as the int8 product takes them.  n_rows: int32 CUDA tensor of one value, the
+    rows in use; the rest are left as they were."""
+    if _elsewhere(x, stream):
+        with _on(x, stream):
+            return quantize_int8(x, act, codes, scales, n_rows)
+    torch = _torch()
+    dt = _dtype(x)
+    x = _in(x, "x", x)
+    rows, cols = x.shape
+    if act == ACT_SWIGLU:
+        if cols % 2:
+            raise FfnError("quantize_int8: ACT_SWIGLU takes an even number of columns")
+        cols //= 2
+    if codes is None:
+        codes = torch.empty(rows, (cols + 15) // 16 * 16, dtype=torch.int8, device=x.device)[:, :cols]
+    else:
+        codes = _out(codes, "codes", x, rows, cols, torch.int8)
+    scales = torch.empty(rows, dtype=torch.float32, device=x.device) if scales is None \
+        else _vec(scales, "scales", x, rows)
+    if n_rows is not None:
+        _vec(n_rows, "n_rows", x, 1, torch.int32)
+    check(lib().ffn_b200_quantize_int8(rows, cols, dt, x.data_ptr(), _ld(x), int(act), _ptr(n_rows),
+                                       codes.data_ptr(), _ld(codes), scales.data_ptr(), _raw(x)),
+          "quantize_int8")
+    return codes, scales
+
+
+class Int8Matrix:
+    """int8 weights on the device, one matrix w [rows, cols] or several experts'
+    [groups, rows, cols], with a scale (and optionally a bias) per output
+    channel, f32 [(groups,) rows].  The rows of w may be padded (slices of wider
+    rows); rows that do not start on 16-byte boundaries are laid out again."""
+
+    def __init__(self, w, scale, bias=None):
+        torch = _torch()
+        if w.dtype != torch.int8 or w.dim() not in (2, 3) or not w.is_cuda or 0 in w.shape:
+            raise FfnError("Int8Matrix: w must be a CUDA int8 tensor [rows, cols] or [groups, rows, cols]")
+        if w.dim() == 2:
+            w = w.unsqueeze(0)
+        self.groups, self.rows, self.cols = w.shape
+        ld = w.stride(1) if self.rows > 1 else (w.stride(0) if self.groups > 1 else self.cols)
+        if self.rows == 1 and self.groups == 1:
+            ld = (self.cols + 15) // 16 * 16  # the stride of a single row is never used
+        if w.data_ptr() % 16 or ld % 16 or ld < self.cols or (self.cols > 1 and w.stride(2) != 1) or \
+                (self.groups > 1 and w.stride(0) != self.rows * ld):
+            ld = (self.cols + 15) // 16 * 16
+            wide = torch.zeros(self.groups, self.rows, ld, dtype=torch.int8, device=w.device)
+            wide[:, :, :self.cols] = w
+            w = wide[:, :, :self.cols]
+        self.w, self.ld = w, ld
+        self.scale = _vec(scale, "scale", w, self.groups * self.rows)
+        self.bias = None if bias is None else _vec(bias, "bias", w, self.groups * self.rows)
+
+    @classmethod
+    def quantize(cls, w, bias=None, stream=None):
+        """Float weights [rows, cols] or [groups, rows, cols], one scale per
+        output channel (ffn_b200_quantize_int8 over the channels)."""
+        if w.dim() not in (2, 3):
+            raise FfnError("Int8Matrix.quantize: w must be [rows, cols] or [groups, rows, cols]")
+        codes, scales = quantize_int8(w.reshape(-1, w.shape[-1]), stream=stream)
+        ld = codes.stride(0) if codes.shape[0] > 1 else (w.shape[-1] + 15) // 16 * 16
+        codes = codes.as_strided(w.shape, ((w.shape[1] * ld, ld, 1) if w.dim() == 3 else (ld, 1)))
+        return cls(codes, scales, bias)
+
+    def matmul(self, x, out=None, offsets=None, dtype=None, stream=None):
+        """out [tokens, rows] = x [tokens, cols] W^T, x float rows (quantised per
+        token first) or their (codes, scales); in `dtype`, by default out's
+        type, x's, or float32 for codes.  Several groups: offsets int32 [groups + 1],
+        tokens offsets[g] .. offsets[g + 1] - 1 take group g, the others' rows
+        are left as they were."""
+        torch = _torch()
+        codes = x[0] if isinstance(x, (tuple, list)) else x
+        if _elsewhere(codes, stream):
+            with _on(codes, stream):
+                return self.matmul(x, out, offsets, dtype)
+        if dtype is None:
+            dtype = out.dtype if out is not None else x.dtype if codes is x else torch.float32
+        if codes is x:
+            x = _in(x, "x", self.w, None, self.cols, x.dtype)
+            n, dt = x.shape[0], _dtype(x)
+            # codes and scales in one buffer
+            ld = (self.cols + 15) // 16 * 16
+            buf = torch.empty(n * (ld + 4), dtype=torch.int8, device=x.device)
+            pc = buf.data_ptr()
+            ps, s = pc + n * ld, _raw(x)
+            check(lib().ffn_b200_quantize_int8(n, self.cols, dt, x.data_ptr(), _ld(x), ACT_NONE, None, pc, ld,
+                                               ps, s), "quantize_int8")
+        else:
+            codes, scales = x
+            codes = _in(codes, "codes", self.w, None, self.cols)
+            n, s = codes.shape[0], _raw(codes)
+            ld = codes.stride(0) if n > 1 else (self.cols + 15) // 16 * 16
+            if ld % 16 or codes.data_ptr() % 16:  # not as quantize_int8 lays them out
+                wide = torch.empty(n, (self.cols + 15) // 16 * 16, dtype=torch.int8, device=codes.device)
+                wide[:, :self.cols] = codes
+                codes, ld = wide, wide.stride(0)
+            pc, ps = codes.data_ptr(), _vec(scales, "scales", codes, n).data_ptr()
+        out = _out(out, "out", self.w, n, self.rows, dtype)
+        if offsets is not None:
+            _vec(offsets, "offsets", out, self.groups + 1, torch.int32)
+        check(lib().ffn_b200_int8_matmul(n, self.rows, self.cols, self.groups, _ptr(offsets), pc, ld, ps,
+                                         self.w.data_ptr(), self.ld, self.scale.data_ptr(), _ptr(self.bias),
+                                         _dtype(out), out.data_ptr(), _ld(out), s), "int8_matmul")
+        return out
+
+    matvec = matmul
+
+    def dequant(self):
+        """f32 weights [(groups,) rows, cols]."""
+        w = self.w.float() * self.scale.view(self.groups, self.rows, 1)
+        return w[0] if self.groups == 1 else w
+
+    def nbytes(self) -> int:
+        return self.groups * self.rows * (self.cols + 4 + (0 if self.bias is None else 4))
+
+
+def moe_sort(idx, expert_begin, expert_end, stream=None):
+    """The routed pairs of idx int32 [tokens, top_k] sorted by expert, those of
+    the experts [expert_begin, expert_end) only: (offsets [experts + 1], pos
+    [tokens, top_k] with -1 elsewhere, src [tokens * top_k] with -1 behind the
+    last row), all int32 (ffn_b200_moe_sort)."""
+    if _elsewhere(idx, stream):
+        with _on(idx, stream):
+            return moe_sort(idx, expert_begin, expert_end)
+    torch = _torch()
+    if idx.dim() != 2 or idx.dtype != torch.int32 or idx.shape[1] == 0:
+        raise FfnError("moe_sort: idx must be int32 [tokens, top_k]")
+    idx = idx.contiguous()
+    n, top_k = idx.shape
+    if expert_end <= expert_begin:
+        raise FfnError("moe_sort: empty expert range")
+    offsets = torch.empty(expert_end - expert_begin + 1, dtype=torch.int32, device=idx.device)
+    pos = torch.empty_like(idx)
+    src = torch.empty(n * top_k, dtype=torch.int32, device=idx.device)
+    check(lib().ffn_b200_moe_sort(n, top_k, idx.data_ptr(), int(expert_begin), int(expert_end),
+                                  offsets.data_ptr(), pos.data_ptr(), src.data_ptr(), _raw(idx)), "moe_sort")
+    return offsets, pos, src
+
+
+def _pos(pos, what, like):
+    if pos.dim() != 2 or pos.shape[1] == 0:
+        raise FfnError(f"{what}: pos must be int32 [tokens, top_k]")
+    return _vec(pos, "pos", like, pos.numel(), _torch().int32)
+
+
+def moe_permute(x, pos, out=None, scales=None, out_scales=None, stream=None):
+    """out[pos[t, k]] = x[t] for rows of any type (ffn_b200_moe_permute); new
+    rows: one per pair.  With scales f32 [tokens] (int8 rows): (out,
+    out_scales).  Rows that no pair names are left as they were."""
+    if _elsewhere(x, stream):
+        with _on(x, stream):
+            return moe_permute(x, pos, out, scales, out_scales)
+    torch = _torch()
+    _pos(pos, "moe_permute", x)
+    n, top_k = pos.shape
+    es = x.element_size()
+    if x.dim() == 2 and x.shape[0] > 1 and x.dtype == torch.int8 and out is None and x.stride(1) == 1 and \
+            x.stride(0) > x.shape[1] and x.stride(0) == (x.shape[1] + 15) // 16 * 16:
+        # codes as quantize_int8 lays them out keep their padded rows
+        out = torch.empty(n * top_k, x.stride(0), dtype=torch.int8, device=x.device)[:, :x.shape[1]]
+    x = _in(x, "x", x, n)
+    cols = x.shape[1]
+    if out is None:
+        out = torch.empty(n * top_k, cols, dtype=x.dtype, device=x.device)
+    else:
+        out = _out(out, "out", x, out.shape[0], cols)
+    if scales is not None:
+        _vec(scales, "scales", x, n)
+        out_scales = torch.empty(out.shape[0], dtype=torch.float32, device=x.device) if out_scales is None \
+            else _vec(out_scales, "out_scales", x, out.shape[0])
+    elif out_scales is not None:
+        raise FfnError("moe_permute: out_scales without scales")
+    check(lib().ffn_b200_moe_permute(n, top_k, cols * es, x.data_ptr(), _ld(x) * es, pos.data_ptr(),
+                                     out.shape[0], out.data_ptr(), _ld(out) * es, _ptr(scales),
+                                     _ptr(out_scales), _raw(x)), "moe_permute")
+    return out if scales is None else (out, out_scales)
+
+
+def moe_combine(y, pos, weight=None, residual=None, out=None, stream=None):
+    """out[t] = residual[t] + sum_k weight[t, k] y[pos[t, k]] (weight f32
+    [tokens, top_k] or None: 1), in f32, rounded once (ffn_b200_moe_combine)."""
+    if _elsewhere(y, stream):
+        with _on(y, stream):
+            return moe_combine(y, pos, weight, residual, out)
+    dt = _dtype(y)
+    _pos(pos, "moe_combine", y)
+    y = _in(y, "y", y)
+    n, cols = pos.shape[0], y.shape[1]
+    if weight is not None:
+        _vec(weight, "weight", y, pos.numel())
+    if residual is not None:
+        residual = _in(residual, "residual", y, n, cols)
+    out = _out(out, "out", y, n, cols)
+    check(lib().ffn_b200_moe_combine(n, pos.shape[1], cols, dt, y.data_ptr(), _ld(y), y.shape[0], pos.data_ptr(),
+                                     _ptr(weight), _ptr(residual), 0 if residual is None else _ld(residual),
+                                     out.data_ptr(), _ld(out), _raw(y)), "moe_combine")
+    return out
+
+
+def moe_combine_backward(dout, y, pos, weight=None, dy=None, stream=None):
+    """Gradients of moe_combine: (dy, dw), dy[pos[t, k]] = weight[t, k] dout[t],
+    dw [tokens, top_k] f32 (ffn_b200_moe_combine_bwd).  The residual's gradient
+    is dout.  A new dy has zeros in the rows that no pair names; in a given one
+    they are left as they were."""
+    if _elsewhere(y, stream):
+        with _on(y, stream):
+            return moe_combine_backward(dout, y, pos, weight, dy)
+    torch = _torch()
+    dt = _dtype(y)
+    _pos(pos, "moe_combine_backward", y)
+    y = _in(y, "y", y)
+    n, (rows, cols) = pos.shape[0], y.shape
+    dout = _in(dout, "dout", y, n, cols)
+    if weight is not None:
+        _vec(weight, "weight", y, pos.numel())
+    dy = torch.zeros(rows, cols, dtype=y.dtype, device=y.device) if dy is None else _out(dy, "dy", y, rows, cols)
+    dw = torch.empty(n, pos.shape[1], dtype=torch.float32, device=y.device)
+    check(lib().ffn_b200_moe_combine_bwd(n, pos.shape[1], cols, dt, dout.data_ptr(), _ld(dout), y.data_ptr(),
+                                         _ld(y), rows, pos.data_ptr(), _ptr(weight), dy.data_ptr(), _ld(dy),
+                                         dw.data_ptr(), _raw(y)), "moe_combine_bwd")
+    return dy, dw
+
+
+def moe_permute_backward(dout, pos, dx=None, stream=None):
+    """Gradient of moe_permute: dx[t] = sum_k dout[pos[t, k]]."""
+    return moe_combine(dout, pos, out=dx, stream=stream)
+
+
+class BlockNorm:
+    """The norms after one block and before the next (ffn_b200_block_norm):
+    h = alpha residual + beta gate rms(y) post_w, xn = rms(h) pre_w.  post_w
+    None: y itself; pre_w None: no xn.  The gate is f32 [cols] (a parameter) or
+    [rows, 1] (one per token)."""
+
+    def __init__(self, pre_w=None, post_w=None, alpha=1.0, beta=1.0, eps=1e-6):
+        self.pre_w, self.post_w = pre_w, post_w
+        self.alpha, self.beta, self.eps = alpha, beta, eps
+
+    def _desc(self, like, rows, cols, gate, post):
+        kind = GATE_NONE
+        if gate is not None:
+            if gate.dim() == 1 and gate.shape[0] == cols:
+                kind = GATE_CHANNEL
+            elif gate.dim() == 2 and tuple(gate.shape) == (rows, 1):
+                kind = GATE_TOKEN
+            else:
+                raise FfnError(f"gate: expected [{cols}] or [{rows}, 1], got {list(gate.shape)}")
+            _vec(gate, "gate", like, gate.numel())
+        post_w = self.post_w if post else None
+        if post_w is not None:
+            _vec(post_w, "post_w", like, cols)
+        if self.pre_w is not None:
+            _vec(self.pre_w, "pre_w", like, cols)
+        return BlockNormDesc(rows, cols, _dtype(like), kind, _ptr(post_w), _ptr(gate), _ptr(self.pre_w),
+                             self.alpha, self.beta, self.eps, 0)
+
+    def forward(self, y, residual=None, gate=None, h=None, xn=None, codes=False, stream=None):
+        """(h, xn), each a new tensor or the one given; y None: the residual
+        alone.  codes True: (h, xn, codes, scales) with xn None unless given and
+        the int8 codes of xn (quantize_int8 of its f32 values)."""
+        like = residual if y is None else y
+        if like is None:
+            raise FfnError("BlockNorm: neither y nor residual")
+        if _elsewhere(like, stream):
+            with _on(like, stream):
+                return self.forward(y, residual, gate, h, xn, codes)
+        torch = _torch()
+        if like.dim() != 2:
+            raise FfnError(f"BlockNorm: expected rows [rows, cols], got {list(like.shape)}")
+        rows, cols = like.shape
+        if y is None and gate is not None:
+            raise FfnError("BlockNorm: a gate without y")
+        d = self._desc(like, rows, cols, gate, y is not None)
+        if y is not None:
+            y = _in(y, "y", like, rows, cols)
+        if residual is not None:
+            residual = _in(residual, "residual", like, rows, cols)
+        h = _out(h, "h", like, rows, cols)
+        q = sc = None
+        if codes:
+            if self.pre_w is None:
+                raise FfnError("BlockNorm: codes need pre_w")
+            q = torch.empty(rows, (cols + 15) // 16 * 16, dtype=torch.int8, device=like.device)[:, :cols]
+            sc = torch.empty(rows, dtype=torch.float32, device=like.device)
+        if xn is not None:
+            xn = _out(xn, "xn", like, rows, cols)
+        elif self.pre_w is not None and not codes:
+            xn = torch.empty(rows, cols, dtype=like.dtype, device=like.device)
+        check(lib().ffn_b200_block_norm(C.byref(d), _ptr(y), 0 if y is None else _ld(y), _ptr(residual),
+                                        0 if residual is None else _ld(residual), h.data_ptr(), _ld(h),
+                                        _ptr(xn), 0 if xn is None else _ld(xn), _ptr(q),
+                                        0 if q is None else _ld(q), _ptr(sc), _raw(like)), "block_norm")
+        return (h, xn, q, sc) if codes else (h, xn)
+
+    def backward(self, y, h, dh=None, dxn=None, gate=None, stream=None):
+        """The gradients, from the y and h of the forward pass and the gradients
+        of h (past the norm) and xn: {"dy", "dres", "dpost_w", "dgate",
+        "dpre_w"}, None where there is no such input."""
+        like = next((t for t in (dxn, dh) if t is not None), None)
+        if like is None:
+            raise FfnError("BlockNorm.backward: neither dh nor dxn")
+        if _elsewhere(like, stream):
+            with _on(like, stream):
+                return self.backward(y, h, dh, dxn, gate)
+        torch = _torch()
+        if like.dim() != 2:
+            raise FfnError(f"BlockNorm.backward: expected rows [rows, cols], got {list(like.shape)}")
+        rows, cols = like.shape
+        if y is None and gate is not None:
+            raise FfnError("BlockNorm.backward: a gate without y")
+        if dxn is not None and (h is None or self.pre_w is None):
+            raise FfnError("BlockNorm.backward: dxn needs h and pre_w")
+        d = self._desc(like, rows, cols, gate, y is not None)
+
+        def row(t, what):
+            return None if t is None else _in(t, what, like, rows, cols)
+        y, h, dh, dxn = row(y, "y"), row(h, "h"), row(dh, "dh"), row(dxn, "dxn")
+
+        def new(on, shape, dtype):
+            return torch.empty(shape, dtype=dtype, device=like.device) if on else None
+        f32 = torch.float32
+        dres = new(True, (rows, cols), like.dtype)
+        dy = new(y is not None, (rows, cols), like.dtype)
+        dpost = new(d.post_w is not None, (cols,), f32)
+        dgate = new(gate is not None, None if gate is None else gate.shape, f32)
+        dpre = new(dxn is not None, (cols,), f32)
+        ws = new(True, (lib().ffn_b200_block_norm_bwd_ws_bytes(C.byref(d)),), torch.uint8)
+
+        def at(t):
+            return (None, 0) if t is None else (t.data_ptr(), _ld(t))
+        check(lib().ffn_b200_block_norm_bwd(C.byref(d), *at(y), *at(h), *at(dh), *at(dxn), *at(dres), *at(dy),
+                                            _ptr(dpost), _ptr(dgate), _ptr(dpre), ws.data_ptr(), ws.numel(),
+                                            _raw(like)), "block_norm_bwd")
+        return {"dy": dy, "dres": dres, "dpost_w": dpost, "dgate": dgate, "dpre_w": dpre}
+
+
+class Int8Experts:
+    """SwiGLU experts in int8 behind a router: gate_up Int8Matrix [experts,
+    2 inter, hidden] (gate channels, then up), down Int8Matrix [experts, hidden,
+    inter], those of the experts [expert_begin, expert_begin + experts) of the
+    routing (expert parallelism: the others' contributions are left out)."""
+
+    def __init__(self, gate_up, down, expert_begin=0):
+        if gate_up.groups != down.groups or gate_up.rows != 2 * down.cols or gate_up.cols != down.rows:
+            raise FfnError("Int8Experts: expected gate_up [experts, 2 inter, hidden] and down "
+                           "[experts, hidden, inter]")
+        self.gate_up, self.down, self.expert_begin = gate_up, down, int(expert_begin)
+
+    def forward(self, x, topk_idx, topk_w, residual=None, out=None, stream=None):
+        """out[t] = residual[t] + sum_k topk_w[t, k] expert(topk_idx[t, k])(x[t]);
+        x float rows [tokens, hidden], or the (codes, scales) of such rows with
+        `residual` or `out` giving the type (float32 without either)."""
+        torch = _torch()
+        first = x[0] if isinstance(x, (tuple, list)) else x
+        if _elsewhere(first, stream):
+            with _on(first, stream):
+                return self.forward(x, topk_idx, topk_w, residual, out)
+        like = next((t for t in (x if first is x else None, residual, out) if t is not None), None)
+        dtype = torch.float32 if like is None else like.dtype
+        codes, scales = quantize_int8(x) if first is x else x
+        offsets, pos, _ = moe_sort(topk_idx, self.expert_begin, self.expert_begin + self.gate_up.groups)
+        rows = moe_permute(codes, pos, scales=scales)
+        gu = self.gate_up.matmul(rows, offsets=offsets, dtype=dtype)
+        act = quantize_int8(gu, ACT_SWIGLU, n_rows=offsets[-1:])
+        y = self.down.matmul(act, offsets=offsets, dtype=dtype)
+        return moe_combine(y, pos, topk_w, residual=residual, out=out)

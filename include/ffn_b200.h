@@ -299,6 +299,128 @@ FFN_B200_EXPORT int ffn_b200_moe_layer(const ffn_b200_moe_desc *d, size_t n_tok,
                                        int32_t *topk_idx, float *topk_w, void *ws,
                                        size_t ws_bytes, void *stream);
 
+/* ------------------------------------------- activation rows of any type
+ * The operators below take rows of f32, bf16 or f16 (`dtype`); strides (ld_*)
+ * count elements unless said otherwise, and rows may be slices of wider ones.
+ * Rows are read 16 bytes at a time where every pointer and stride allows it,
+ * else element by element.  Sums are f32, results round once to `dtype`. */
+#define FFN_B200_DT_F32 0
+#define FFN_B200_DT_BF16 1
+#define FFN_B200_DT_F16 2
+
+/* ------------------------------------------------------- int8 products
+ * Dynamically quantised activations times int8 weights, one scale per token and
+ * one per output channel (the reference's row-scaled int8 matrices, HA:22-76,
+ * with both sides in 8 bits).
+ *
+ * quantize_int8: per row, scale = fl32(max|x| / 127) and codes = fl32(x / scale)
+ * rounded to the nearest whole number (ties to even), within +-127.  A row of
+ * zeros: scale 0, codes 0.  A row with an infinity or a NaN: scale NaN, codes 0,
+ * so that its products are NaN.  act SWIGLU: x rows hold cols gate values, then
+ * cols up values, and min(silu(gate), 10) * clamp(up, -10, 10) is quantised
+ * (flash1017.rs:7539).  n_rows: DEVICE count of the rows in use (the last of
+ * moe_sort's offsets) or NULL; rows behind it are neither read nor written.
+ * codes [rows][ld_codes]; cols <= 16384.  Also quantises weights: a row per
+ * output channel. */
+#define FFN_B200_ACT_NONE 0
+#define FFN_B200_ACT_SWIGLU 1
+FFN_B200_EXPORT int ffn_b200_quantize_int8(size_t rows, size_t cols, int32_t dtype, const void *x, size_t ld_x,
+                                           int32_t act, const int32_t *n_rows, int8_t *codes, size_t ld_codes,
+                                           float *scales, void *stream);
+/* out[r][j] = x_scales[r] * w_scales[g][j] * sum_i x[r][i] w[g][j][i] + bias[g][j],
+ * the sum exact in int32 (k <= 131072), out in dtype.  x [rows][ld_x] codes, w
+ * [n_groups][n][ld_w] codes (groups contiguous), w_scales and bias (or NULL)
+ * [n_groups][n] f32.  offsets DEVICE [n_groups + 1]: group g has the rows
+ * offsets[g] .. offsets[g + 1] - 1, as moe_sort writes them (ascending; values
+ * outside 0..rows are clamped); NULL: one group of all rows.  Rows in no group
+ * are left as they were.  x, w 16-byte aligned, ld_x and ld_w multiples of 16;
+ * any n and k (bytes of a row behind k are not used).  At most 4096 groups; no
+ * workspace.  A wait inside the kernel that runs out writes NaN. */
+FFN_B200_EXPORT int ffn_b200_int8_matmul(size_t rows, size_t n, size_t k, size_t n_groups, const int32_t *offsets,
+                                         const int8_t *x, size_t ld_x, const float *x_scales, const int8_t *w,
+                                         size_t ld_w, const float *w_scales, const float *bias, int32_t dtype,
+                                         void *out, size_t ld_out, void *stream);
+
+/* --------------------------------------------- routed pairs: sort and back
+ * The layer's grouping and combine (flash1017.rs:8088-8099, 8267-8326) as
+ * operators of their own, for experts that the caller runs itself, with their
+ * gradients.
+ *
+ * moe_sort: the pairs p = t * top_k + k of idx [n_tok][top_k] whose expert is in
+ * [expert_begin, expert_end) (at most 4096 experts), ordered by expert and by p
+ * inside an expert.  offsets [expert_end - expert_begin + 1]: first row of each
+ * expert, then the number of rows.  pos [n_tok][top_k] (or NULL): each pair's
+ * row, -1 outside the range (the top-k step's 0x7fffffff included).  src
+ * [n_tok * top_k] (or NULL): each row's pair, -1 behind the last row.  All
+ * DEVICE; at most 2^30 pairs; no workspace. */
+FFN_B200_EXPORT int ffn_b200_moe_sort(size_t n_tok, size_t top_k, const int32_t *idx, int32_t expert_begin,
+                                      int32_t expert_end, int32_t *offsets, int32_t *pos, int32_t *src,
+                                      void *stream);
+/* out[pos[t][k]] = x[t]: rows of row_bytes bytes, ld_x and ld_out in BYTES, any
+ * type; with x_scale [n_tok] also out_scale[pos[t][k]] = x_scale[t] (int8 rows and
+ * their scales).  Pairs with pos outside [0, out_rows) are skipped, rows that no
+ * pair names are left as they were.  out must not overlap x. */
+FFN_B200_EXPORT int ffn_b200_moe_permute(size_t n_tok, size_t top_k, size_t row_bytes, const void *x,
+                                         size_t ld_x, const int32_t *pos, size_t out_rows, void *out,
+                                         size_t ld_out, const float *x_scale, float *out_scale, void *stream);
+/* out[t] = residual[t] + sum_k w[t][k] * y[pos[t][k]], k in order; residual and w
+ * may be NULL (0 and 1); pairs with pos outside [0, y_rows) add nothing.  out may
+ * be residual, not y.  Without w and residual: the gradient of moe_permute. */
+FFN_B200_EXPORT int ffn_b200_moe_combine(size_t n_tok, size_t top_k, size_t cols, int32_t dtype, const void *y,
+                                         size_t ld_y, size_t y_rows, const int32_t *pos, const float *w,
+                                         const void *residual, size_t ld_res, void *out, size_t ld_out,
+                                         void *stream);
+/* The gradient of moe_combine: dy[pos[t][k]] = w[t][k] * dout[t] (w NULL: 1) and
+ * dw[t][k] = sum of dout[t] * y[pos[t][k]] (0 where pos is outside [0, y_rows));
+ * either of dy, dw may be NULL, y too without dw.  Rows of dy that no pair names
+ * are left as they were.  The residual's gradient is dout. */
+FFN_B200_EXPORT int ffn_b200_moe_combine_bwd(size_t n_tok, size_t top_k, size_t cols, int32_t dtype,
+                                             const void *dout, size_t ld_dout, const void *y, size_t ld_y,
+                                             size_t y_rows, const int32_t *pos, const float *w, void *dy,
+                                             size_t ld_dy, float *dw, void *stream);
+
+/* ------------------------------------- norms after and before a block
+ * With rms(v) = v / sqrt(mean(v^2) + eps), the reference's norm
+ * (flash1017.rs:4880-4891):
+ *   b  = rms(y) * post_w          (y itself when post_w is NULL)
+ *   h  = alpha * residual + beta * gate * b
+ *   xn = rms(h) * pre_w
+ * y is a block's output, h the residual stream behind it, xn the next block's
+ * input.  cols <= 16384; eps >= 0. */
+#define FFN_B200_GATE_NONE 0
+#define FFN_B200_GATE_CHANNEL 1 /* gate [cols] */
+#define FFN_B200_GATE_TOKEN 2   /* gate [rows] */
+typedef struct ffn_b200_block_norm_desc {
+    size_t rows, cols;
+    int32_t dtype;      /* FFN_B200_DT_* of all rows */
+    int32_t gate_kind;  /* FFN_B200_GATE_* */
+    const float *post_w; /* DEVICE [cols] or NULL */
+    const float *gate;   /* DEVICE, by gate_kind, or NULL */
+    const float *pre_w;  /* DEVICE [cols] or NULL (no xn) */
+    float alpha, beta, eps;
+    uint32_t reserved;
+} ffn_b200_block_norm_desc;
+/* y or residual may be NULL (0); h, xn and codes are written where non-NULL.  codes
+ * [rows][ld_codes] int8 with code_scales [rows]: the f32 values of xn, quantised
+ * as ffn_b200_quantize_int8 does.  h may be y or residual; other outputs must
+ * not overlap inputs. */
+FFN_B200_EXPORT int ffn_b200_block_norm(const ffn_b200_block_norm_desc *d, const void *y, size_t ld_y,
+                                        const void *residual, size_t ld_res, void *h, size_t ld_h, void *xn,
+                                        size_t ld_xn, int8_t *codes, size_t ld_codes, float *code_scales,
+                                        void *stream);
+/* The gradient.  y and h as the forward pass read and stored them; dh: the
+ * gradient that reaches h past the norm, dxn: that of xn (either may be NULL, h
+ * too without dxn).  dresidual, dy [rows][cols] in dtype, dpost_w [cols], dgate
+ * (by gate_kind), dpre_w [cols] in f32, each written where non-NULL.  dresidual
+ * may be dh, and dy may be y or dxn; else outputs must not overlap inputs or each
+ * other.  ws: only with dpost_w, dpre_w or a per-channel dgate. */
+FFN_B200_EXPORT size_t ffn_b200_block_norm_bwd_ws_bytes(const ffn_b200_block_norm_desc *d);
+FFN_B200_EXPORT int ffn_b200_block_norm_bwd(const ffn_b200_block_norm_desc *d, const void *y, size_t ld_y,
+                                            const void *h, size_t ld_h, const void *dh, size_t ld_dh,
+                                            const void *dxn, size_t ld_dxn, void *dresidual, size_t ld_dres,
+                                            void *dy, size_t ld_dy, float *dpost_w, float *dgate, float *dpre_w,
+                                            void *ws, size_t ws_bytes, void *stream);
+
 /* ----------------------------------------------- seeded synthetic weights
  * Counter-based generators (SplitMix64 finaliser + Irwin-Hall normals +
  * round-to-nearest-even E4M3), byte-identical to the CPU oracle's.  NVFP4 w
@@ -344,7 +466,11 @@ FFN_B200_EXPORT int ffn_b200_dequant_ternary(size_t rows, size_t cols, const uin
 #define FFN_B200_K_QUANT 14       /* activation rows -> six NVFP4 terms (FP4 path) */
 #define FFN_B200_K_FP4_GATEUP 15  /* block-scaled FP4 tensor-core path */
 #define FFN_B200_K_FP4_DOWN 16
-#define FFN_B200_K_COUNT 17
+#define FFN_B200_K_ROUTE 17       /* moe_sort, moe_permute, moe_combine and its gradient */
+#define FFN_B200_K_NORM 18        /* block_norm and its gradient */
+#define FFN_B200_K_INT8_QUANT 19  /* activation rows -> int8 codes */
+#define FFN_B200_K_INT8_GEMM 20   /* int8 product */
+#define FFN_B200_K_COUNT 21
 FFN_B200_EXPORT int ffn_b200_profile_enable(int enable);
 /* Which kinds get event pairs while enabled: bit k = FFN_B200_K_* k (default
  * all).  Timing fewer kinds puts fewer event records between the kernels. */
