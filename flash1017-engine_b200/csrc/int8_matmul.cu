@@ -23,6 +23,11 @@
 namespace ffn {
 namespace i8 {
 
+// The output of one sum: the same operations wherever it is formed.
+__device__ __forceinline__ float product_value(int acc, float s, float sw, float bias) {
+  return fmaf((float)acc * s, sw, bias);
+}
+
 // ---------------------------------------------------------------- quantise
 struct QuantArgs {
   const void *x;
@@ -34,14 +39,15 @@ struct QuantArgs {
   uint32_t cols, n_vec;
 };
 
-// The framework's gated activation (flash1017.rs:7539) of gate g and up u.
+// The framework's gated activation (flash1017.rs:7539) of gate g and up u; the
+// fast division is within 2 steps, and gives the limit 0 where exp(-g) leaves f32.
 __device__ __forceinline__ float swiglu10(float g, float u) {
-  return fminf(g / (1.0f + expf(-g)), 10.0f) * fminf(fmaxf(u, -10.0f), 10.0f);
+  return fminf(__fdividef(g, 1.0f + expf(-g)), 10.0f) * fminf(fmaxf(u, -10.0f), 10.0f);
 }
 
 template <typename T, int VEC, int NV, bool WARP, bool SWIGLU>
 __global__ void __launch_bounds__(WARP ? 256 : 1024) quant_kernel(const QuantArgs a) {
-  __shared__ float s_red[32];
+  __shared__ uint32_t s_red[32];
   pdl_enter();
   const uint32_t l = WARP ? threadIdx.x & 31 : threadIdx.x, L = WARP ? 32 : blockDim.x;
   const long long row = WARP ? (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
@@ -56,44 +62,44 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) quant_kernel(const QuantArg
       if (SWIGLU) ru[i] = load_raw<T, VEC>(xr + a.cols, v);
     }
   }
-  float f[NV][VEC];
-  float amax = 0.f;
-  bool fin = true;
+  float f[SWIGLU ? NV : 1][VEC];
+  uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const uint32_t v = l + i * L;
-    if (v < a.n_vec) {
+    if (v >= a.n_vec) continue;
+    if (SWIGLU) {
+      float u[VEC];
       unpack<T, VEC>(rx[i], f[i]);
-      if (SWIGLU) {
-        float u[VEC];
-        unpack<T, VEC>(ru[i], u);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          fin = fin && isfinite(f[i][j]) && isfinite(u[j]);
-          f[i][j] = swiglu10(f[i][j], u[j]);
-        }
-      }
+      unpack<T, VEC>(ru[i], u);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        fin = fin && isfinite(f[i][j]);
-        amax = fmaxf(amax, fabsf(f[i][j]));
+        // the clamps would hide a gate or an up that is not finite
+        const bool fin = isfinite(f[i][j]) && isfinite(u[j]);
+        f[i][j] = swiglu10(f[i][j], u[j]);
+        m = max(m, fin ? __float_as_uint(f[i][j]) & 0x7fffffffu : 0x7f800000u);
       }
+    } else {
+      m = max(m, abs_bits<T, VEC>(rx[i]));
     }
   }
-  amax = warp_max(fin ? amax : INFINITY);
+  m = __reduce_max_sync(0xffffffffu, m);
   if (!WARP) {
     const int lane = threadIdx.x & 31, nw = blockDim.x >> 5;
-    if (lane == 0) s_red[threadIdx.x >> 5] = amax;
+    if (lane == 0) s_red[threadIdx.x >> 5] = m;
     __syncthreads();
-    amax = warp_max(lane < nw ? s_red[lane] : 0.f);
+    m = __reduce_max_sync(0xffffffffu, lane < nw ? s_red[lane] : 0u);
   }
-  const float sc = int8_scale(amax);
+  const Int8Row sc(SWIGLU ? __uint_as_float(m) : from_abs_bits<T>(m));
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const uint32_t v = l + i * L;
-    if (v < a.n_vec) store_codes<VEC>(a.codes + (size_t)row * a.ld_c + (size_t)v * VEC, f[i], sc);
+    if (v >= a.n_vec) continue;
+    float e[VEC];
+    if (!SWIGLU) unpack<T, VEC>(rx[i], e);
+    store_codes<VEC>(a.codes + (size_t)row * a.ld_c + (size_t)v * VEC, SWIGLU ? f[SWIGLU ? i : 0] : e, sc);
   }
-  if (l == 0) a.scales[row] = sc;
+  if (l == 0) a.scales[row] = sc.scale();
 }
 
 // ----------------------------------------------------------------- product
@@ -341,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
         for (int j = 0; j < 16; ++j) {
           const float s = __shfl_sync(0xffffffffu, sx, j);
           // a wait that ran out leaves NaN behind
-          const float f = ok ? (float)(int)v[j] * s * sw + bias : __int_as_float(0x7fffffff);
+          const float f = ok ? product_value((int)v[j], s, sw, bias) : __int_as_float(0x7fffffff);
           if (on && c + j < o.nn) out[(size_t)(c + j) * a.ld_out] = ToF32<T>::put(f);
         }
       }
@@ -363,8 +369,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
         if (ch >= a.n) continue;
         int acc = 0;
         for (int q = 0; q < a.cs; ++q) acc += red[(q * a.nt + r) * own + c];
-        float f = (float)acc * __ldg(a.xs + o.r0 + r) * __ldg(a.ws + (size_t)o.g * a.n + ch);
-        if (a.bias) f += __ldg(a.bias + (size_t)o.g * a.n + ch);
+        float f = product_value(acc, __ldg(a.xs + o.r0 + r), __ldg(a.ws + (size_t)o.g * a.n + ch),
+                                a.bias ? __ldg(a.bias + (size_t)o.g * a.n + ch) : 0.f);
         if (s_err) f = __int_as_float(0x7fffffff);
         reinterpret_cast<T *>(a.out)[(size_t)(o.r0 + r) * a.ld_out + ch] = ToF32<T>::put(f);
       }
@@ -376,6 +382,151 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
     tc::fence_after();
     tc::dealloc(tmem, tmem_cols);
   }
+}
+
+// ------------------------------------------- few tokens, quantised in place
+// A decode step of 1 to 4 tokens against one matrix: a single launch.  Every CTA
+// quantises the tokens for itself (a few KB, L2 hits) while its warps' first
+// weights are on the way; a warp then takes a channel at a time, 16 bytes a
+// lane and load, and multiplies with dp4a.  Bound by the weights' bytes: 128 KB
+// of loads in flight an SM.
+constexpr int kFewRows = 4;
+constexpr int kFewThreads = 256;
+constexpr size_t kFewSmem = 47 * 1024;  // the launch default, less the static part
+struct FewArgs {
+  const void *x;
+  size_t ld_x, ld_w, ld_out;
+  const int8_t *w;
+  const float *ws, *bias;
+  void *out;
+  int n, k, out_dtype;
+  bool x16;  // x's rows can be read 16 bytes at a time
+};
+__host__ __device__ constexpr int few_pitch(int k) { return (k + 4095) / 4096 * 4096; }  // code bytes a token
+
+// 16 weights from column 16 p of a row (zeros past k)
+__device__ __forceinline__ uint4 few_piece(const int8_t *row, int p, int k) {
+  if (16 * p + 16 <= k) return ldg_stream(row + 16 * p);
+  union { uint4 v; int8_t b[16]; } u;
+  u.v = make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (16 * p + i < k) u.b[i] = __ldg(row + 16 * p + i);
+  return u.v;
+}
+
+template <typename T, int R>
+__global__ void __launch_bounds__(kFewThreads) few_kernel(const FewArgs a) {
+  constexpr int VEC = 16 / sizeof(T);
+  extern __shared__ __align__(16) int8_t s_codes[];  // [R][few_pitch(k)]
+  __shared__ uint32_t s_max[R][kFewThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int kWarps = kFewThreads / 32;
+  const int pitch = few_pitch(a.k), step = gridDim.x * kWarps;
+  int c = blockIdx.x * kWarps + warp;
+  // while the previous kernel drains: a hint only, nothing is read
+  if (c < a.n && lane * 128 < a.k)
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(a.w + (size_t)c * a.ld_w + lane * 128));
+  pdl_enter();
+  uint4 w[8];
+  auto load = [&](int ch, int base) {  // the 4096 bytes from column `base`
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int p = base / 16 + lane + 32 * j;
+      w[j] = make_uint4(0, 0, 0, 0);
+      if (ch < a.n && 16 * p < a.k) w[j] = few_piece(a.w + (size_t)ch * a.ld_w, p, a.k);
+    }
+  };
+  load(c, 0);
+
+  // quantise: largest magnitudes, then codes
+  uint32_t m[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    m[r] = 0;
+    const T *x = (const T *)a.x + (size_t)r * a.ld_x;
+    if (a.x16)
+      for (int v = tid; v * VEC < a.k; v += kFewThreads) m[r] = max(m[r], abs_bits<T, VEC>(load_raw<T, VEC>(x, v)));
+    else
+      for (int v = tid; v < a.k; v += kFewThreads) m[r] = max(m[r], abs_bits<T, 1>(load_raw<T, 1>(x, v)));
+    m[r] = __reduce_max_sync(0xffffffffu, m[r]);
+    if (lane == 0) s_max[r][warp] = m[r];
+  }
+  __syncthreads();
+  float scale[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const Int8Row sc(from_abs_bits<T>(__reduce_max_sync(0xffffffffu, lane < kWarps ? s_max[r][lane] : 0u)));
+    scale[r] = sc.scale();
+    const T *x = (const T *)a.x + (size_t)r * a.ld_x;
+    int8_t *q = s_codes + r * pitch;
+    if (a.x16) {
+      for (int v = tid; v * VEC < pitch; v += kFewThreads) {
+        float e[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) e[j] = 0.f;
+        if (v * VEC < a.k) unpack<T, VEC>(load_raw<T, VEC>(x, v), e);
+        store_codes<VEC>(q + v * VEC, e, sc);
+      }
+    } else {
+      for (int v = tid; v < pitch; v += kFewThreads) {
+        float e[1] = {0.f};
+        if (v < a.k) unpack<T, 1>(load_raw<T, 1>(x, v), e);
+        store_codes<1>(q + v, e, sc);
+      }
+    }
+  }
+  __syncthreads();
+
+  for (; c < a.n; c += step) {
+    int acc[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) acc[r] = 0;
+    for (int base = 0; base < a.k; base += 4096) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (base + 512 * j >= a.k) break;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const uint4 q = *reinterpret_cast<const uint4 *>(s_codes + r * pitch + base + 16 * (lane + 32 * j));
+          acc[r] = __dp4a((int)w[j].x, (int)q.x, acc[r]);
+          acc[r] = __dp4a((int)w[j].y, (int)q.y, acc[r]);
+          acc[r] = __dp4a((int)w[j].z, (int)q.z, acc[r]);
+          acc[r] = __dp4a((int)w[j].w, (int)q.w, acc[r]);
+        }
+      }
+      if (base + 4096 < a.k) load(c, base + 4096);
+      else load(c + step, 0);
+    }
+    const float sw = __ldg(a.ws + c), bias = a.bias ? __ldg(a.bias + c) : 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int sum = __reduce_add_sync(0xffffffffu, acc[r]);
+      const float f = product_value(sum, scale[r], sw, bias);
+      if (lane == r) {
+        const size_t at = (size_t)r * a.ld_out + c;
+        if (a.out_dtype == FFN_B200_DT_F32) ((float *)a.out)[at] = f;
+        else if (a.out_dtype == FFN_B200_DT_BF16) ((__nv_bfloat16 *)a.out)[at] = ToF32<__nv_bfloat16>::put(f);
+        else ((__half *)a.out)[at] = ToF32<__half>::put(f);
+      }
+    }
+  }
+}
+
+template <typename T>
+int launch_few(const FewArgs &a, int rows, int sms, cudaStream_t st) {
+  const int grid = std::min((a.n + kFewThreads / 32 - 1) / (kFewThreads / 32), sms * 4);
+  const size_t smem = (size_t)rows * few_pitch(a.k);
+#define FFN_GO(R) FFN_LAUNCH_PDL(FFN_B200_K_INT8_GEMM, st, "int8_linear", (few_kernel<T, R>), grid, kFewThreads, smem, a)
+  if (rows == 1) FFN_GO(1);
+  else if (rows == 2) FFN_GO(2);
+  else if (rows == 3) FFN_GO(3);
+  else FFN_GO(4);
+#undef FFN_GO
+  return 0;
+}
+bool few_fits(size_t rows, size_t k, size_t n_groups, const int32_t *offsets) {
+  return rows <= (size_t)kFewRows && n_groups == 1 && !offsets && k <= 16384 && rows * few_pitch((int)k) <= kFewSmem;
 }
 
 // ------------------------------------------------------------------ launch
@@ -439,6 +590,71 @@ int launch_gemm(const GemmArgs &a, int grid, size_t smem, const CUtensorMap &mw,
   return 0;
 }
 
+// Checks a product and lays out its launch (p.grid 0: nothing to do).
+struct GemmPlan {
+  GemmArgs a;
+  CUtensorMap mw, mx;
+  size_t smem;
+  int grid, dev;
+};
+int plan_gemm(GemmPlan &p, size_t rows, size_t n, size_t k, size_t n_groups, const int32_t *offsets, const int8_t *x,
+              size_t ld_x, const float *x_scales, const int8_t *w, size_t ld_w, const float *w_scales, const float *bias,
+              int32_t dtype, void *out, size_t ld_out) {
+  p.grid = 0;
+  if (!dtype_ok(dtype)) return fail(FFN_B200_EINVAL, "int8_matmul: unknown dtype");
+  if (n == 0 || k == 0 || k > 131072) return fail(FFN_B200_EUNSUP, "int8 product: n must be positive and k in 1..131072");
+  if (n_groups == 0 || n_groups > 4096) return fail(FFN_B200_EINVAL, "int8_matmul: n_groups must be in 1..4096");
+  if (n_groups > 1 && !offsets) return fail(FFN_B200_EINVAL, "int8_matmul: several groups need offsets");
+  if (rows > (1u << 30) || n > (1u << 30) / n_groups) return fail(FFN_B200_EINVAL, "int8_matmul: too many rows");
+  if (rows == 0) return 0;
+  if (!x || !x_scales || !w || !w_scales || !out) return fail(FFN_B200_EINVAL, "int8_matmul: null pointer");
+  if (((uintptr_t)x | (uintptr_t)w | ld_x | ld_w) % 16)
+    return fail(FFN_B200_EINVAL, "int8_matmul: x, w and their row strides must be multiples of 16 bytes");
+  if (ld_x < k || ld_w < k || (rows > 1 && ld_out < n)) return fail(FFN_B200_EINVAL, "int8_matmul: rows overlap");
+  if ((uintptr_t)out % dtype_bytes(dtype) || ((uintptr_t)x_scales | (uintptr_t)w_scales | (uintptr_t)bias) % 4)
+    return fail(FFN_B200_EINVAL, "int8_matmul: out and scales must be aligned to their type");
+  FFN_CUDA_TRY(cudaGetDevice(&p.dev));
+  const int dev = p.dev;
+  if (dev < 0 || dev >= 64) return fail(FFN_B200_EUNSUP, "int8_matmul: device index >= 64");
+  const int sms = sm_count_of(dev);
+  GemmArgs &a = p.a;
+  a = GemmArgs{};
+  a.offsets = offsets;
+  a.xs = x_scales, a.ws = w_scales, a.bias = bias;
+  a.out = out, a.ld_out = ld_out;
+  a.rows = (int)rows, a.n = (int)n, a.groups = (int)n_groups;
+  a.kt = (int)((k + kKB - 1) / kKB);
+  // tokens a tile: the smallest that holds an average group (a third on top for
+  // uneven ones)
+  const size_t avg = offsets ? (rows + n_groups - 1) / n_groups * 4 / 3 : rows;
+  a.nt = avg <= 16 ? 16 : avg <= 32 ? 32 : avg <= 64 ? 64 : avg <= 128 ? 128 : 256;
+  a.bx = std::min(a.nt, 64);
+  const long long ct = (long long)((n + kM - 1) / kM);
+  // tiles at most: each group may end in a partial chunk
+  const long long chunks = offsets ? std::min<long long>(rows, rows / a.nt + n_groups) : (rows + a.nt - 1) / a.nt;
+  const long long tiles = ct * chunks;
+  // (the kernel's tile numbers stay in 32 bits even where offsets are not ascending)
+  if ((double)(rows / a.nt + 1) * (double)n_groups * (double)ct > 2147483647.0) return fail(FFN_B200_EINVAL, "int8_matmul: too many tiles");
+  // few tiles: K split over a cluster
+  a.cs = 1;
+  if (a.nt <= 64)
+    while (a.cs < 8 && tiles * a.cs * 2 <= sms && a.kt >= 4 * a.cs) a.cs *= 2;
+  const size_t tail = (a.cs > 1 ? (size_t)kM * a.nt * 4 : 0) + (3 * n_groups + 1) * sizeof(int);
+  const size_t stage = (size_t)kABytes + (size_t)a.nt * kKB;
+  a.stages = (int)std::min<size_t>({(kSmemMax - 1024 - tail) / stage, (size_t)kMaxStages, (size_t)std::max(2, a.kt)});
+  if (a.stages < 2) return fail(FFN_B200_EUNSUP, "int8_matmul: too many groups for shared memory");
+  p.smem = 1024 + a.stages * stage + tail;
+  if (int rc = encode(&p.mw, w, n_groups * n, k, ld_w, kM)) return rc;
+  if (int rc = encode(&p.mx, x, rows, k, ld_x, a.bx)) return rc;
+  p.grid = a.cs > 1 ? (int)tiles * a.cs : (int)std::min<long long>(tiles, sms);
+  return 0;
+}
+int run_gemm(const GemmPlan &p, int32_t dtype, cudaStream_t st) {
+  if (dtype == FFN_B200_DT_F32) return launch_gemm<float>(p.a, p.grid, p.smem, p.mw, p.mx, p.dev, st);
+  if (dtype == FFN_B200_DT_BF16) return launch_gemm<__nv_bfloat16>(p.a, p.grid, p.smem, p.mw, p.mx, p.dev, st);
+  return launch_gemm<__half>(p.a, p.grid, p.smem, p.mw, p.mx, p.dev, st);
+}
+
 template <typename T, int VEC, bool SWIGLU>
 int launch_quant(QuantArgs &a, cudaStream_t st) {
   a.n_vec = a.cols / VEC;
@@ -496,56 +712,59 @@ int ffn_b200_int8_matmul(size_t rows, size_t n, size_t k, size_t n_groups, const
                          size_t ld_x, const float *x_scales, const int8_t *w, size_t ld_w, const float *w_scales,
                          const float *bias, int32_t dtype, void *out, size_t ld_out, void *stream) {
   using namespace ffn::i8;
-  if (!dtype_ok(dtype)) return fail(FFN_B200_EINVAL, "int8_matmul: unknown dtype");
-  if (n == 0 || k == 0 || k > 131072) return fail(FFN_B200_EUNSUP, "int8_matmul: n must be positive and k in 1..131072");
-  if (n_groups == 0 || n_groups > 4096) return fail(FFN_B200_EINVAL, "int8_matmul: n_groups must be in 1..4096");
-  if (n_groups > 1 && !offsets) return fail(FFN_B200_EINVAL, "int8_matmul: several groups need offsets");
-  if (rows > (1u << 30) || n > (1u << 30) / n_groups) return fail(FFN_B200_EINVAL, "int8_matmul: too many rows");
+  GemmPlan p;
+  if (int rc = plan_gemm(p, rows, n, k, n_groups, offsets, x, ld_x, x_scales, w, ld_w, w_scales, bias, dtype, out, ld_out))
+    return rc;
+  return p.grid ? run_gemm(p, dtype, (cudaStream_t)stream) : 0;
+}
+
+size_t ffn_b200_int8_linear_ws_bytes(size_t rows, size_t k, size_t n_groups, const int32_t *offsets) {
+  if (ffn::i8::few_fits(rows, k, n_groups, offsets)) return 0;
+  return rows * ((k + 15) / 16 * 16 + sizeof(float));
+}
+
+int ffn_b200_int8_linear(size_t rows, size_t n, size_t k, size_t n_groups, const int32_t *offsets, int32_t x_dtype,
+                         const void *x, size_t ld_x, const int8_t *w, size_t ld_w, const float *w_scales, const float *bias,
+                         int32_t dtype, void *out, size_t ld_out, void *ws, size_t ws_bytes, void *stream) {
+  using namespace ffn::i8;
+  if (!dtype_ok(x_dtype) || !dtype_ok(dtype)) return fail(FFN_B200_EINVAL, "int8_linear: unknown dtype");
+  if (n == 0 || k == 0 || k > 16384) return fail(FFN_B200_EUNSUP, "int8_linear: n must be positive and k in 1..16384");
+  if (!few_fits(rows, k, n_groups, offsets)) {
+    const size_t ld = (k + 15) / 16 * 16;
+    if (rows > (1u << 30)) return fail(FFN_B200_EINVAL, "int8_linear: too many rows");
+    if (rows && (!ws || (uintptr_t)ws % 16)) return fail(FFN_B200_EINVAL, "int8_linear: the workspace is null or misaligned");
+    if (ws_bytes < rows * (ld + sizeof(float))) return fail(FFN_B200_ENOSPC, "int8_linear: workspace too small");
+    int8_t *codes = (int8_t *)ws;
+    float *scales = (float *)(codes + rows * ld);
+    GemmPlan p;
+    if (int rc = plan_gemm(p, rows, n, k, n_groups, offsets, codes, ld, scales, w, ld_w, w_scales, bias, dtype, out, ld_out))
+      return rc;
+    // rows behind the last group's are in no product: not quantised either
+    if (int rc = ffn_b200_quantize_int8(rows, k, x_dtype, x, ld_x, FFN_B200_ACT_NONE, offsets ? offsets + n_groups : nullptr,
+                                        codes, ld, scales, stream))
+      return rc;
+    return p.grid ? run_gemm(p, dtype, (cudaStream_t)stream) : 0;
+  }
   if (rows == 0) return 0;
-  if (!x || !x_scales || !w || !w_scales || !out) return fail(FFN_B200_EINVAL, "int8_matmul: null pointer");
-  if (((uintptr_t)x | (uintptr_t)w | ld_x | ld_w) % 16)
-    return fail(FFN_B200_EINVAL, "int8_matmul: x, w and their row strides must be multiples of 16 bytes");
-  if (ld_x < k || ld_w < k || (rows > 1 && ld_out < n)) return fail(FFN_B200_EINVAL, "int8_matmul: rows overlap");
-  if ((uintptr_t)out % dtype_bytes(dtype) || ((uintptr_t)x_scales | (uintptr_t)w_scales | (uintptr_t)bias) % 4)
-    return fail(FFN_B200_EINVAL, "int8_matmul: out and scales must be aligned to their type");
+  if (!x || !w || !w_scales || !out) return fail(FFN_B200_EINVAL, "int8_linear: null pointer");
+  if (((uintptr_t)w | ld_w) % 16) return fail(FFN_B200_EINVAL, "int8_linear: w and its row stride must be multiples of 16 bytes");
+  if (n > (1u << 30)) return fail(FFN_B200_EINVAL, "int8_linear: too many channels");
+  if (ld_w < k || (rows > 1 && (ld_out < n || ld_x < k))) return fail(FFN_B200_EINVAL, "int8_linear: rows overlap");
+  const size_t es = dtype_bytes(x_dtype);
+  if ((uintptr_t)x % es || (uintptr_t)out % dtype_bytes(dtype) || ((uintptr_t)w_scales | (uintptr_t)bias) % 4)
+    return fail(FFN_B200_EINVAL, "int8_linear: rows and scales must be aligned to their type");
+  FewArgs a{};
+  a.x = x, a.ld_x = ld_x, a.w = w, a.ld_w = ld_w, a.ws = w_scales, a.bias = bias;
+  a.out = out, a.ld_out = ld_out, a.out_dtype = dtype;
+  a.n = (int)n, a.k = (int)k;
+  a.x16 = k * es % 16 == 0 && rows16(x, ld_x, es);
   int dev = 0;
   FFN_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64) return fail(FFN_B200_EUNSUP, "int8_matmul: device index >= 64");
   const int sms = sm_count_of(dev);
-  GemmArgs a{};
-  a.offsets = offsets;
-  a.xs = x_scales, a.ws = w_scales, a.bias = bias;
-  a.out = out, a.ld_out = ld_out;
-  a.rows = (int)rows, a.n = (int)n, a.groups = (int)n_groups;
-  a.kt = (int)((k + kKB - 1) / kKB);
-  // tokens a tile: the smallest that holds an average group (a third on top for
-  // uneven ones)
-  const size_t avg = offsets ? (rows + n_groups - 1) / n_groups * 4 / 3 : rows;
-  a.nt = avg <= 16 ? 16 : avg <= 32 ? 32 : avg <= 64 ? 64 : avg <= 128 ? 128 : 256;
-  a.bx = std::min(a.nt, 64);
-  const long long ct = (long long)((n + kM - 1) / kM);
-  // tiles at most: each group may end in a partial chunk
-  const long long chunks = offsets ? std::min<long long>(rows, rows / a.nt + n_groups) : (rows + a.nt - 1) / a.nt;
-  const long long tiles = ct * chunks;
-  // (the kernel's tile numbers stay in 32 bits even where offsets are not ascending)
-  if ((double)(rows / a.nt + 1) * (double)n_groups * (double)ct > 2147483647.0) return fail(FFN_B200_EINVAL, "int8_matmul: too many tiles");
-  // few tiles: K split over a cluster
-  a.cs = 1;
-  if (a.nt <= 64)
-    while (a.cs < 8 && tiles * a.cs * 2 <= sms && a.kt >= 4 * a.cs) a.cs *= 2;
-  const size_t tail = (a.cs > 1 ? (size_t)kM * a.nt * 4 : 0) + (3 * n_groups + 1) * sizeof(int);
-  const size_t stage = (size_t)kABytes + (size_t)a.nt * kKB;
-  a.stages = (int)std::min<size_t>({(kSmemMax - 1024 - tail) / stage, (size_t)kMaxStages, (size_t)std::max(2, a.kt)});
-  if (a.stages < 2) return fail(FFN_B200_EUNSUP, "int8_matmul: too many groups for shared memory");
-  const size_t smem = 1024 + a.stages * stage + tail;
-  CUtensorMap mw, mx;
-  if (int rc = encode(&mw, w, n_groups * n, k, ld_w, kM)) return rc;
-  if (int rc = encode(&mx, x, rows, k, ld_x, a.bx)) return rc;
-  const int grid = a.cs > 1 ? (int)tiles * a.cs : (int)std::min<long long>(tiles, sms);
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == FFN_B200_DT_F32) return launch_gemm<float>(a, grid, smem, mw, mx, dev, st);
-  if (dtype == FFN_B200_DT_BF16) return launch_gemm<__nv_bfloat16>(a, grid, smem, mw, mx, dev, st);
-  return launch_gemm<__half>(a, grid, smem, mw, mx, dev, st);
+  if (x_dtype == FFN_B200_DT_F32) return launch_few<float>(a, (int)rows, sms, st);
+  if (x_dtype == FFN_B200_DT_BF16) return launch_few<__nv_bfloat16>(a, (int)rows, sms, st);
+  return launch_few<__half>(a, (int)rows, sms, st);
 }
 
 }  // extern "C"

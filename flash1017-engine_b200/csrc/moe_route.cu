@@ -21,15 +21,18 @@ namespace route {
 
 // ------------------------------------------------------------------- sort
 // A stable counting sort in one launch: one thread-block cluster, each warp a
-// contiguous segment of the pairs.  A warp ranks 32 pairs at a time with
-// match.any (lanes of the same expert, in lane order), so the order inside an
-// expert is the pair order.  Counts per (segment, expert) sit in shared
+// contiguous segment of the pairs.  A warp ranks 32 pairs at a time (the lanes
+// with the same expert, found by a ballot per bit of the expert number, in lane
+// order), so the order inside an expert is the pair order.  match.any finds the
+// same lanes in one instruction, but its latency was most of the kernel's time
+// (49152 pairs: 20 us).  Counts per (segment, expert) sit in shared
 // memory; the CTAs of the cluster read each other's totals over distributed
 // shared memory, which saves the second and third launch and the workspace
 // that a grid-wide sort would need.  Bound by latency, not by bytes: 8 bytes
 // a pair.
 constexpr int kSortThreads = 1024;
-constexpr int kSortCluster = 8;
+constexpr int kSortCluster = 16;    // most CTAs of a cluster (8 are portable)
+constexpr int kSortBatch = 8;
 constexpr int kSortCounts = 32768;  // (segments per CTA) x (local experts): 128 KB of counters
 
 struct SortArgs {
@@ -55,9 +58,20 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 __device__ __forceinline__ int peer_int(const int *p, uint32_t rank) {
   uint32_t a = (uint32_t)__cvta_generic_to_shared(p), b;
   int v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(a), "r"(rank));
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(b) : "memory");
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(a), "r"(rank));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(b));
   return v;
+}
+
+// the lanes whose v (below 2^bits) is this lane's
+__device__ __forceinline__ uint32_t same_lanes(uint32_t v, int bits) {
+  uint32_t m = 0xffffffffu;
+  for (int b = 0; b < bits; ++b) {
+    const bool one = v >> b & 1u;
+    const uint32_t set = __ballot_sync(0xffffffffu, one);
+    m &= one ? set : ~set;
+  }
+  return m;
 }
 
 __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortArgs a) {
@@ -68,37 +82,54 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortArgs a)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = cluster_rank(), nrank = cluster_size();
   int *tot = s_cnt + a.segs * a.n_local, *off = tot + a.n_local;
-  for (int i = tid; i < a.segs * a.n_local; i += kSortThreads) s_cnt[i] = 0;
-  __syncthreads();
-
-  // pass 1: counts per segment
+  // pass 1: counts per segment.  kSortBatch groups of ids are asked for before the
+  // first is ranked (one at a time, 49152 pairs took 15 us, most of it latency).
   const long long s0 = ((long long)rank * a.segs + warp) * a.per_seg;
   const int p0 = (int)min(s0, (long long)a.n_pairs), p1 = (int)min(s0 + a.per_seg, (long long)a.n_pairs);
   int *mine = s_cnt + warp * a.n_local;
-  if (warp < a.segs) {
-    for (int p = p0; p < p1; p += 32) {
-      int e = -1;
-      if (p + lane < p1) {
+  auto ids = [&](int p, int (&e)[kSortBatch]) {
+#pragma unroll
+    for (int i = 0; i < kSortBatch; ++i) {
+      e[i] = -1;
+      if (p + 32 * i + lane < p1) {
         // unsigned: ids below e_begin, and the top-k step's "no candidate"
         // 0x7fffffff, fall outside like those at or above the range's end
-        const uint32_t r = (uint32_t)__ldg(a.idx + p + lane) - (uint32_t)a.e_begin;
-        if (r < (uint32_t)a.n_local) e = (int)r;
+        const uint32_t r = (uint32_t)__ldg(a.idx + p + 32 * i + lane) - (uint32_t)a.e_begin;
+        if (r < (uint32_t)a.n_local) e[i] = (int)r;
       }
-      const uint32_t same = __match_any_sync(0xffffffffu, e);
-      if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
-      __syncwarp();
+    }
+  };
+  int e[kSortBatch], rk[kSortBatch];  // rk: the pair's number inside its expert and segment
+  const int bits = 32 - __clz(a.n_local);
+  if (warp < a.segs) ids(p0, e);
+  for (int i = tid; i < a.segs * a.n_local; i += kSortThreads) s_cnt[i] = 0;
+  __syncthreads();
+  if (warp < a.segs) {
+    for (int p = p0; p < p1; p += 32 * kSortBatch) {
+      if (p > p0) ids(p, e);
+#pragma unroll
+      for (int i = 0; i < kSortBatch; ++i) {
+        if (p + 32 * i >= p1) break;
+        const uint32_t same = same_lanes(e[i] < 0 ? a.n_local : e[i], bits);
+        const int base = e[i] >= 0 ? mine[e[i]] : 0;
+        rk[i] = base + __popc(same & ((1u << lane) - 1u));
+        __syncwarp();
+        if (e[i] >= 0 && lane == __ffs(same) - 1) mine[e[i]] = base + __popc(same);
+        __syncwarp();
+      }
     }
   }
   __syncthreads();
   // counts -> exclusive prefix over this CTA's segments; totals
-  for (int e = tid; e < a.n_local; e += kSortThreads) {
+  for (int x = tid; x < a.n_local; x += kSortThreads) {
     int run = 0;
+#pragma unroll 8
     for (int s = 0; s < a.segs; ++s) {
-      const int c = s_cnt[s * a.n_local + e];
-      s_cnt[s * a.n_local + e] = run;
+      const int c = s_cnt[s * a.n_local + x];
+      s_cnt[s * a.n_local + x] = run;
       run += c;
     }
-    tot[e] = run;
+    tot[x] = run;
   }
   __syncthreads();  // the cluster barrier is .aligned: whole warps arrive
   cluster_arrive();
@@ -107,15 +138,19 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortArgs a)
   // lower-ranked CTAs come first inside an expert
   if (tid == 0) s_carry = 0;
   __syncthreads();
-  for (int e0 = 0; e0 < a.n_local; e0 += kSortThreads) {
-    const int e = e0 + tid;
+  for (int x0 = 0; x0 < a.n_local; x0 += kSortThreads) {
+    const int x = x0 + tid;
     int all = 0, before = 0;
-    if (e < a.n_local)
-      for (uint32_t r = 0; r < nrank; ++r) {
-        const int c = r == rank ? tot[e] : peer_int(tot + e, r);
-        all += c;
-        if (r < rank) before += c;
+    if (x < a.n_local) {
+      int c[kSortCluster];
+#pragma unroll
+      for (uint32_t r = 0; r < kSortCluster; ++r) c[r] = r < nrank ? peer_int(tot + x, r) : 0;
+#pragma unroll
+      for (uint32_t r = 0; r < kSortCluster; ++r) {
+        all += c[r];
+        if (r < rank) before += c[r];
       }
+    }
     int inc = all;
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, inc, o);
@@ -133,9 +168,9 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortArgs a)
     }
     __syncthreads();
     const int first = s_carry + (warp ? s_warp[warp - 1] : 0) + inc - all;
-    if (e < a.n_local) {
-      off[e] = first + before;
-      if (rank == 0) a.offsets[e] = first;
+    if (x < a.n_local) {
+      off[x] = first + before;
+      if (rank == 0) a.offsets[x] = first;
     }
     __syncthreads();
     if (tid == 0) s_carry += s_warp[31];
@@ -145,23 +180,28 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortArgs a)
   if (rank == 0 && tid == 0) a.offsets[a.n_local] = total;
   cluster_arrive();  // the reads of the peers' totals are done; waited for at the end
 
-  // pass 2: rows
+  // pass 2: rows.  One batch (up to 256 pairs a segment) is still in registers with
+  // its numbers; longer segments are ranked again.
   if (warp < a.segs) {
-    for (int p = p0; p < p1; p += 32) {
-      int e = -1;
-      if (p + lane < p1) {
-        const uint32_t r = (uint32_t)__ldg(a.idx + p + lane) - (uint32_t)a.e_begin;
-        if (r < (uint32_t)a.n_local) e = (int)r;
-      }
-      const uint32_t same = __match_any_sync(0xffffffffu, e);
-      const int base = e >= 0 ? mine[e] : 0;
-      __syncwarp();
-      if (e >= 0 && lane == __ffs(same) - 1) mine[e] = base + __popc(same);
-      __syncwarp();
-      const int row = e >= 0 ? off[e] + base + __popc(same & ((1u << lane) - 1u)) : -1;
-      if (p + lane < p1) {
-        if (a.pos) a.pos[p + lane] = row;
-        if (a.src && row >= 0) a.src[row] = p + lane;
+    const bool kept = a.per_seg <= 32 * kSortBatch;
+    for (int p = p0; p < p1; p += 32 * kSortBatch) {
+      if (!kept) ids(p, e);
+#pragma unroll
+      for (int i = 0; i < kSortBatch; ++i) {
+        if (p + 32 * i >= p1) break;
+        const int at = p + 32 * i + lane, first = e[i] >= 0 ? mine[e[i]] : 0;
+        if (!kept) {
+          const uint32_t same = same_lanes(e[i] < 0 ? a.n_local : e[i], bits);
+          rk[i] = __popc(same & ((1u << lane) - 1u));
+          __syncwarp();
+          if (e[i] >= 0 && lane == __ffs(same) - 1) mine[e[i]] = first + __popc(same);
+          __syncwarp();
+        }
+        const int row = e[i] >= 0 ? off[e[i]] + first + rk[i] : -1;
+        if (at < p1) {
+          if (a.pos) a.pos[at] = row;
+          if (a.src && row >= 0) a.src[row] = at;
+        }
       }
     }
   }
@@ -172,88 +212,118 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortArgs a)
   cluster_wait();
 }
 
-// (row, piece) of flat item i; 32-bit division where the items allow it
-__device__ __forceinline__ int split_item(long long i, uint32_t n_vec, bool small, uint32_t &v) {
-  if (small) {
-    const uint32_t t = (uint32_t)i / n_vec;
-    v = (uint32_t)i - t * n_vec;
-    return (int)t;
+// src from pos, for many pairs: their scattered 4-byte stores take one SM 32
+// cycles a warp, which the sort's 8 CTAs cannot hide (49152 pairs: 12.0 us with
+// src written by the sort, 11.0 us with this kernel behind it).
+constexpr int kSrcPairs = 16384;
+__global__ void __launch_bounds__(256) src_kernel(const int32_t *pos, const int32_t *total, int32_t *src, int n_pairs) {
+  pdl_enter();
+  const int n = __ldg(total);
+  for (int p = blockIdx.x * 256 + threadIdx.x; p < n_pairs; p += gridDim.x * 256) {
+    const uint32_t r = (uint32_t)__ldg(pos + p);
+    if (r < (uint32_t)n_pairs) src[r] = p;
+    if (p >= n) src[p] = -1;
   }
-  const long long t = i / n_vec;
-  v = (uint32_t)(i - t * n_vec);
-  return (int)t;
 }
 
+// Work layout of the row kernels: `tpt` threads (a power of two, 32 .. 256) share
+// a token, a CTA of 256 holds 256 / tpt tokens; a warp works on one token, its
+// lanes hold the token's pos and weights (choice k in lane k % 32) and hand them
+// round by shuffles.  The next token's are loaded while this one's rows move, so
+// that the chain of two DRAM latencies (pos, then rows) is not paid per token.
+
 // ------------------------------------------------- permute (rows of bytes)
-// Flat over (token, piece of BYTES): each piece is read once and written to
-// the token's rows.  DRAM-bound by the written rows.
+// blockIdx.y cuts long rows into segments of tpt * kPieces pieces; each piece is
+// read once and written to the token's rows.  DRAM-bound by the written rows
+// (stores alone reach 6.7 TB/s on this GPU).
+constexpr int kPieces = 4;
 template <int BYTES>
 __global__ void __launch_bounds__(256) permute_kernel(const uint8_t *x, size_t ld_x, const int32_t *pos, uint8_t *out,
                                                       size_t ld_out, int n_tok, int top_k, uint32_t n_vec,
-                                                      uint32_t out_rows, const float *x_scale, float *out_scale) {
+                                                      uint32_t out_rows, const float *x_scale, float *out_scale, int tpt) {
   using R = typename RawOf<BYTES>::type;
   pdl_enter();
-  const long long total = (long long)n_tok * n_vec, step = (long long)gridDim.x * 256;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
-    uint32_t v;
-    const int t = split_item(i, n_vec, total <= 0xffffffffLL, v);
-    const R r = reinterpret_cast<const R *>(x + (size_t)t * ld_x)[v];
-    const float s = x_scale && v == 0 ? __ldg(x_scale + t) : 0.f;
-    const int32_t *pp = pos + (size_t)t * top_k;
+  const int l = threadIdx.x & (tpt - 1), per = 256 / tpt, lane = threadIdx.x & 31;
+  const uint32_t v0 = blockIdx.y * (uint32_t)(tpt * kPieces) + l;
+  const long long step = (long long)gridDim.x * per;
+  long long t = (long long)blockIdx.x * per + threadIdx.x / tpt;
+  auto lookup = [&](long long tok, int k) { return tok < n_tok && k < top_k ? __ldg(pos + (size_t)tok * top_k + k) : -1; };
+  int32_t next = lookup(t, lane);
+  for (; t < n_tok; t += step) {
+    int32_t pl = next;
+    next = lookup(t + step, lane);
+    R r[kPieces];
+    const R *xr = reinterpret_cast<const R *>(x + (size_t)t * ld_x);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+      if (v0 + i * tpt < n_vec) r[i] = xr[v0 + i * tpt];
+    const float s = x_scale && v0 == 0 ? __ldg(x_scale + t) : 0.f;
     for (int k = 0; k < top_k; ++k) {
-      const uint32_t p = (uint32_t)__ldg(pp + k);
+      if (k && (k & 31) == 0) pl = lookup(t, k + lane);
+      const uint32_t p = (uint32_t)__shfl_sync(0xffffffffu, pl, k & 31);
       if (p >= out_rows) continue;
-      reinterpret_cast<R *>(out + (size_t)p * ld_out)[v] = r;
-      if (x_scale && v == 0) out_scale[p] = s;
+      R *o = reinterpret_cast<R *>(out + (size_t)p * ld_out);
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i)
+        if (v0 + i * tpt < n_vec) o[v0 + i * tpt] = r[i];
+      if (x_scale && v0 == 0) out_scale[p] = s;
     }
   }
 }
 
 // ----------------------------------------------------------------- combine
-// Flat over (token, piece of VEC elements); kAhead rows are loaded before the
-// first is used.  DRAM-bound by the experts' rows.
-constexpr int kAhead = 4;
-template <typename T, int VEC>
-__global__ void __launch_bounds__(256) combine_rows_kernel(const T *y, size_t ld_y, uint32_t y_rows, const int32_t *pos,
-                                                           const float *w, const T *residual, size_t ld_r, T *out,
-                                                           size_t ld_o, int n_tok, int top_k, uint32_t n_vec) {
+// A thread's piece of AHEAD routed rows is loaded before the first is used.
+// DRAM-bound by the experts' rows, so what counts is loads on their way: with 6
+// ahead 64 registers are enough and 1024 threads an SM fit (8 ahead and 768
+// threads: 24576 rows of 4096 bf16 took 68 us, 3.4 TB/s).
+template <typename T, int VEC, int AHEAD>
+__global__ void __launch_bounds__(256, AHEAD > 6 ? 3 : 4) combine_rows_kernel(const T *y, size_t ld_y, uint32_t y_rows, const int32_t *pos,
+                                                              const float *w, const T *residual, size_t ld_r, T *out,
+                                                              size_t ld_o, int n_tok, int top_k, uint32_t n_vec, int tpt) {
   pdl_enter();
-  const long long total = (long long)n_tok * n_vec, step = (long long)gridDim.x * 256;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
-    uint32_t v;
-    const int t = split_item(i, n_vec, total <= 0xffffffffLL, v);
-    const int32_t *pp = pos + (size_t)t * top_k;
-    const float *ww = w ? w + (size_t)t * top_k : nullptr;
+  const int l = threadIdx.x & (tpt - 1), per = 256 / tpt, lane = threadIdx.x & 31;
+  const uint32_t v = blockIdx.y * (uint32_t)tpt + l;
+  const bool on = v < n_vec;
+  const long long step = (long long)gridDim.x * per;
+  long long t = (long long)blockIdx.x * per + threadIdx.x / tpt;
+  auto lookup = [&](long long tok, int k) { return tok < n_tok && k < top_k ? __ldg(pos + (size_t)tok * top_k + k) : -1; };
+  auto weight = [&](long long tok, int k) { return w && tok < n_tok && k < top_k ? __ldg(w + (size_t)tok * top_k + k) : 1.f; };
+  int32_t next = lookup(t, lane);
+  float next_w = weight(t, lane);
+  for (; t < n_tok; t += step) {
+    int32_t pl = next;
+    float wl = next_w;
+    next = lookup(t + step, lane);
+    next_w = weight(t + step, lane);
     Raw<T, VEC> rr = {};
-    if (residual) rr = load_raw<T, VEC>(residual + (size_t)t * ld_r, v);
+    if (residual && on) rr = load_raw<T, VEC>(residual + (size_t)t * ld_r, v);
     float acc[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
-    for (int k0 = 0; k0 < top_k; k0 += kAhead) {
-      Raw<T, VEC> r[kAhead];
-      float f[kAhead];
-      bool on[kAhead];
+    for (int k0 = 0; k0 < top_k; k0 += AHEAD) {
+      if (k0 && (k0 & 31) == 0) pl = lookup(t, k0 + lane), wl = weight(t, k0 + lane);
+      Raw<T, VEC> r[AHEAD];
+      uint32_t use = 0;
 #pragma unroll
-      for (int q = 0; q < kAhead; ++q) {
-        on[q] = false;
-        if (k0 + q < top_k) {
-          const uint32_t p = (uint32_t)__ldg(pp + k0 + q);
-          on[q] = p < y_rows;
-          if (on[q]) {
-            r[q] = load_raw<T, VEC>(y + (size_t)p * ld_y, v);
-            f[q] = ww ? __ldg(ww + k0 + q) : 1.f;
-          }
+      for (int q = 0; q < AHEAD; ++q) {
+        const uint32_t p = (uint32_t)__shfl_sync(0xffffffffu, pl, (k0 + q) & 31);
+        if (k0 + q < top_k && p < y_rows) {
+          use |= 1u << q;
+          if (on) r[q] = load_raw<T, VEC>(y + (size_t)p * ld_y, v);
         }
       }
 #pragma unroll
-      for (int q = 0; q < kAhead; ++q)
-        if (on[q]) {
+      for (int q = 0; q < AHEAD; ++q) {
+        const float f = __shfl_sync(0xffffffffu, wl, (k0 + q) & 31);
+        if (on && (use >> q & 1u)) {
           float e[VEC];
           unpack<T, VEC>(r[q], e);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) acc[j] = fmaf(f[q], e[j], acc[j]);
+          for (int j = 0; j < VEC; ++j) acc[j] = fmaf(f, e[j], acc[j]);
         }
+      }
     }
+    if (!on) continue;
     if (residual) {
       float e[VEC];
       unpack<T, VEC>(rr, e);
@@ -266,50 +336,52 @@ __global__ void __launch_bounds__(256) combine_rows_kernel(const T *y, size_t ld
 
 // ------------------------------------------------------- combine, backward
 // TPT threads (one warp, or the CTA) a token: the token's gradient row is read
-// once per kBack choices, each choice's row of y once, each row of dy written
-// once; the kBack dot products are reduced together.
-constexpr int kBack = 8;
+// once per kBack choices (again from L1), each choice's row of y once, each row
+// of dy written once; the kBack dot products are reduced together.  kBack = 8
+// took 150 registers, one CTA an SM (4096 tokens x 6 x 4096 bf16, with dx: 193
+// us; 4: 149 us).
+constexpr int kBack = 4;
 template <typename T, int VEC, int TPT>
-__global__ void __launch_bounds__(256) combine_bwd_kernel(const T *dout, size_t ld_d, const T *y, size_t ld_y,
+__global__ void __launch_bounds__(256, 3) combine_bwd_kernel(const T *dout, size_t ld_d, const T *y, size_t ld_y,
                                                           uint32_t y_rows, const int32_t *pos, const float *w, T *dy,
                                                           size_t ld_dy, float *dw, int n_tok, int top_k, uint32_t n_vec) {
   constexpr int kTok = 256 / TPT;
-  __shared__ float s_red[8][kBack];
+  __shared__ float s_red[2][8][kBack];
   pdl_enter();
-  const int lane = threadIdx.x % TPT, sub = threadIdx.x / TPT;
-  for (long long t0 = (long long)blockIdx.x * kTok; t0 < n_tok; t0 += (long long)gridDim.x * kTok) {
-    const long long t = t0 + sub;
-    const bool live = t < n_tok;
-    const int32_t *pp = pos + (size_t)(live ? t : 0) * top_k;
-    const float *ww = w ? w + (size_t)(live ? t : 0) * top_k : nullptr;
-    const T *drow = dout + (size_t)(live ? t : 0) * ld_d;
-    for (int k0 = 0; k0 < top_k; k0 += kBack) {
+  const int l = threadIdx.x % TPT, lane = threadIdx.x & 31;
+  const long long step = (long long)gridDim.x * kTok;
+  long long t = (long long)blockIdx.x * kTok + threadIdx.x / TPT;
+  auto lookup = [&](long long tok, int k) { return tok < n_tok && k < top_k ? __ldg(pos + (size_t)tok * top_k + k) : -1; };
+  auto weight = [&](long long tok, int k) { return w && tok < n_tok && k < top_k ? __ldg(w + (size_t)tok * top_k + k) : 1.f; };
+  int32_t next = lookup(t, lane);
+  float next_w = weight(t, lane);
+  int par = 0;
+  for (; t < n_tok; t += step) {
+    int32_t pl = next;
+    float wl = next_w;
+    next = lookup(t + step, lane);
+    next_w = weight(t + step, lane);
+    const T *drow = dout + (size_t)t * ld_d;
+    for (int k0 = 0; k0 < top_k; k0 += kBack, par ^= 1) {
+      if (k0 && (k0 & 31) == 0) pl = lookup(t, k0 + lane), wl = weight(t, k0 + lane);
       uint32_t p[kBack];
       float f[kBack], dot[kBack];
 #pragma unroll
       for (int q = 0; q < kBack; ++q) {
-        p[q] = live && k0 + q < top_k ? (uint32_t)__ldg(pp + k0 + q) : 0xffffffffu;
-        if (p[q] >= y_rows) p[q] = 0xffffffffu;
-        f[q] = ww && p[q] != 0xffffffffu ? __ldg(ww + k0 + q) : 1.f;
+        p[q] = (uint32_t)__shfl_sync(0xffffffffu, pl, (k0 + q) & 31);
+        if (k0 + q >= top_k || p[q] >= y_rows) p[q] = 0xffffffffu;
+        f[q] = __shfl_sync(0xffffffffu, wl, (k0 + q) & 31);
         dot[q] = 0.f;
       }
-      for (uint32_t v = lane; live && v < n_vec; v += TPT) {
-        float d[VEC];
-        unpack<T, VEC>(load_raw<T, VEC>(drow, v), d);
+      for (uint32_t v = l; v < n_vec; v += TPT) {
+        Raw<T, VEC> r[kBack];
         if (dw) {
-          Raw<T, VEC> r[kBack];
 #pragma unroll
           for (int q = 0; q < kBack; ++q)
             if (p[q] != 0xffffffffu) r[q] = load_raw<T, VEC>(y + (size_t)p[q] * ld_y, v);
-#pragma unroll
-          for (int q = 0; q < kBack; ++q)
-            if (p[q] != 0xffffffffu) {
-              float e[VEC];
-              unpack<T, VEC>(r[q], e);
-#pragma unroll
-              for (int j = 0; j < VEC; ++j) dot[q] = fmaf(d[j], e[j], dot[q]);
-            }
         }
+        float d[VEC];
+        unpack<T, VEC>(load_raw<T, VEC>(drow, v), d);
         if (dy) {
 #pragma unroll
           for (int q = 0; q < kBack; ++q)
@@ -320,23 +392,32 @@ __global__ void __launch_bounds__(256) combine_bwd_kernel(const T *dout, size_t 
               store_vec<T, VEC>(dy + (size_t)p[q] * ld_dy, v, e);
             }
         }
+        if (dw) {
+#pragma unroll
+          for (int q = 0; q < kBack; ++q)
+            if (p[q] != 0xffffffffu) {
+              float e[VEC];
+              unpack<T, VEC>(r[q], e);
+#pragma unroll
+              for (int j = 0; j < VEC; ++j) dot[q] = fmaf(d[j], e[j], dot[q]);
+            }
+        }
       }
       if (dw) {
 #pragma unroll
         for (int q = 0; q < kBack; ++q) dot[q] = warp_sum(dot[q]);
         if (TPT > 32) {
-          if ((threadIdx.x & 31) == 0)
+          if (lane == 0)
 #pragma unroll
-            for (int q = 0; q < kBack; ++q) s_red[threadIdx.x >> 5][q] = dot[q];
-          __syncthreads();
-          if (threadIdx.x < kBack && live && k0 + (int)threadIdx.x < top_k) {
+            for (int q = 0; q < kBack; ++q) s_red[par][threadIdx.x >> 5][q] = dot[q];
+          __syncthreads();  // par: the next sums go elsewhere, so one barrier a round
+          if (threadIdx.x < kBack && k0 + (int)threadIdx.x < top_k) {
             float s = 0.f;
 #pragma unroll
-            for (int g = 0; g < 8; ++g) s += s_red[g][threadIdx.x];
+            for (int g = 0; g < 8; ++g) s += s_red[par][g][threadIdx.x];
             dw[(size_t)t * top_k + k0 + threadIdx.x] = s;
           }
-          __syncthreads();
-        } else if (live) {
+        } else {
 #pragma unroll
           for (int q = 0; q < kBack; ++q)
             if (lane == q && k0 + q < top_k) dw[(size_t)t * top_k + k0 + q] = dot[q];
@@ -347,30 +428,58 @@ __global__ void __launch_bounds__(256) combine_bwd_kernel(const T *dout, size_t 
 }
 
 // ------------------------------------------------------------------ launch
-int flat_grid(long long items) {  // 256 items a CTA, four waves of 8 CTAs an SM at most
+// CTAs for the work, `resident` an SM at most (each then takes several tokens and
+// looks the next one up in time).
+int grid_of(long long ctas, int resident) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
-  return (int)std::max(1LL, std::min<long long>((items + 255) / 256, (long long)sm_count_of(dev) * 32));
+  return (int)std::max(1LL, std::min<long long>(ctas, (long long)sm_count_of(dev) * resident));
+}
+// Threads a token: the most of 256, 128, 64, 32 that leaves at most a tenth of
+// them without a piece in the row's last segment.
+int threads_per_token(uint32_t n_vec, int pieces) {
+  for (int t = 256; t > 32; t /= 2) {
+    const uint64_t seg = (n_vec + (uint64_t)t * pieces - 1) / ((uint64_t)t * pieces);
+    if (seg * t * pieces * 10 <= (uint64_t)n_vec * 11) return t;
+  }
+  return 32;
 }
 
 template <int BYTES>
 int launch_permute(const void *x, size_t ld_x, const int32_t *pos, void *out, size_t ld_out, size_t n_tok, size_t top_k,
                    size_t row_bytes, size_t out_rows, const float *xs, float *os, cudaStream_t st) {
   const uint32_t n_vec = (uint32_t)(row_bytes / BYTES);
-  FFN_LAUNCH_PDL(FFN_B200_K_ROUTE, st, "permute_kernel", (permute_kernel<BYTES>), flat_grid((long long)n_tok * n_vec), 256, 0,
-                 (const uint8_t *)x, ld_x, pos, (uint8_t *)out, ld_out, (int)n_tok, (int)top_k, n_vec, (uint32_t)out_rows,
-                 xs, os);
+  int tpt = threads_per_token(n_vec, 1);
+  const uint32_t seg = (n_vec + tpt * kPieces - 1) / (tpt * kPieces);
+  if (seg > 65535) return fail(FFN_B200_EUNSUP, "moe_permute: row too long for its alignment");
+  const dim3 grid(grid_of((long long)(n_tok + 256 / tpt - 1) / (256 / tpt), std::max<int>(1, 32 / seg)), seg);
+  FFN_LAUNCH_PDL(FFN_B200_K_ROUTE, st, "permute_kernel", (permute_kernel<BYTES>), grid, 256, 0, (const uint8_t *)x, ld_x, pos,
+                 (uint8_t *)out, ld_out, (int)n_tok, (int)top_k, n_vec, (uint32_t)out_rows, xs, os, tpt);
   return 0;
 }
 
+template <typename T, int VEC, int AHEAD>
+int launch_combine_as(const void *y, size_t ld_y, size_t y_rows, const int32_t *pos, const float *w, const void *res,
+                      size_t ld_r, void *out, size_t ld_o, size_t n_tok, size_t top_k, size_t cols, cudaStream_t st) {
+  const uint32_t n_vec = (uint32_t)(cols / VEC);
+  const int tpt = threads_per_token(n_vec, 1);
+  const uint32_t seg = (n_vec + tpt - 1) / tpt;
+  if (seg > 65535) return fail(FFN_B200_EUNSUP, "moe_combine: row too long for its alignment");
+  const dim3 grid(grid_of((long long)(n_tok + 256 / tpt - 1) / (256 / tpt), 32), seg);
+  FFN_LAUNCH_PDL(FFN_B200_K_ROUTE, st, "combine_rows_kernel", (combine_rows_kernel<T, VEC, AHEAD>), grid, 256, 0, (const T *)y,
+                 ld_y, (uint32_t)y_rows, pos, w, (const T *)res, ld_r, (T *)out, ld_o, (int)n_tok, (int)top_k, n_vec, tpt);
+  return 0;
+}
+// rows loaded ahead: all of a token's up to 8; a batch never straddles the 32
+// choices that a warp's lanes hold
 template <typename T, int VEC>
 int launch_combine_rows(const void *y, size_t ld_y, size_t y_rows, const int32_t *pos, const float *w, const void *res,
                         size_t ld_r, void *out, size_t ld_o, size_t n_tok, size_t top_k, size_t cols, cudaStream_t st) {
-  const uint32_t n_vec = (uint32_t)(cols / VEC);
-  FFN_LAUNCH_PDL(FFN_B200_K_ROUTE, st, "combine_rows_kernel", (combine_rows_kernel<T, VEC>),
-                 flat_grid((long long)n_tok * n_vec), 256, 0, (const T *)y, ld_y, (uint32_t)y_rows, pos, w, (const T *)res,
-                 ld_r, (T *)out, ld_o, (int)n_tok, (int)top_k, n_vec);
-  return 0;
+#define FFN_CALL(A) launch_combine_as<T, VEC, A>(y, ld_y, y_rows, pos, w, res, ld_r, out, ld_o, n_tok, top_k, cols, st)
+  if (top_k <= 4) return FFN_CALL(4);
+  if (top_k <= 6) return FFN_CALL(6);
+  return FFN_CALL(8);
+#undef FFN_CALL
 }
 
 template <typename T, int VEC>
@@ -380,12 +489,12 @@ int launch_combine_bwd(const void *dout, size_t ld_d, const void *y, size_t ld_y
   const uint32_t n_vec = (uint32_t)(cols / VEC);
   // a warp a token up to 4 pieces a lane; a CTA a token above
   if (n_vec <= 128) {
-    const int grid = flat_grid((long long)n_tok * 32);
+    const int grid = grid_of((long long)(n_tok + 7) / 8, 3);
     FFN_LAUNCH_PDL(FFN_B200_K_ROUTE, st, "combine_bwd_kernel", (combine_bwd_kernel<T, VEC, 32>), grid, 256, 0,
                    (const T *)dout, ld_d, (const T *)y, ld_y, (uint32_t)y_rows, pos, w, (T *)dy, ld_dy, dw, (int)n_tok,
                    (int)top_k, n_vec);
   } else {
-    const int grid = flat_grid((long long)n_tok * 256);
+    const int grid = grid_of((long long)n_tok, 3);
     FFN_LAUNCH_PDL(FFN_B200_K_ROUTE, st, "combine_bwd_kernel", (combine_bwd_kernel<T, VEC, 256>), grid, 256, 0,
                    (const T *)dout, ld_d, (const T *)y, ld_y, (uint32_t)y_rows, pos, w, (T *)dy, ld_dy, dw, (int)n_tok,
                    (int)top_k, n_vec);
@@ -426,19 +535,39 @@ int ffn_b200_moe_sort(size_t n_tok, size_t top_k, const int32_t *idx, int32_t ex
   a.n_local = expert_end - expert_begin;
   a.offsets = offsets;
   a.pos = pos;
-  a.src = src;
-  // One CTA up to 2048 pairs (two groups of 32 a warp): no cluster to gather.
-  const int nclu = a.n_pairs <= 2048 ? 1 : kSortCluster;
+  const bool later = src && pos && a.n_pairs > kSrcPairs;
+  a.src = later ? nullptr : src;
+  // One CTA up to 512 pairs (384 experts: 4.5 us for 384 pairs, but 7.3 us for 2046
+  // against 4.8 us with the cluster).
+  // Above 8192 pairs 16 CTAs (49152 pairs: 11.0 us with 8, 9.8 us), where this
+  // GPU can hold such a cluster.
+  static int widest[64] = {0};
+  if (!widest[dev]) {
+    FFN_CUDA_TRY(cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (kSortCounts + 2 * 4096) * (int)sizeof(int)));
+    FFN_CUDA_TRY(cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    cudaLaunchAttribute ca;
+    ca.id = cudaLaunchAttributeClusterDimension;
+    ca.val.clusterDim.x = kSortCluster;
+    ca.val.clusterDim.y = ca.val.clusterDim.z = 1;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(kSortCluster);
+    c.blockDim = dim3(kSortThreads);
+    c.dynamicSmemBytes = (kSortCounts + 2 * 4096) * sizeof(int);
+    c.attrs = &ca;
+    c.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, sort_kernel, &c) != cudaSuccess) {
+      (void)cudaGetLastError();
+      n = 0;
+    }
+    widest[dev] = n > 0 ? kSortCluster : 8;
+  }
+  const int nclu = a.n_pairs <= 512 ? 1 : a.n_pairs <= 8192 ? 8 : widest[dev];
   const int groups = (a.n_pairs + 31) / 32, per_cta = (groups + nclu - 1) / nclu;
   a.segs = std::max(1, std::min({kSortThreads / 32, kSortCounts / a.n_local, per_cta}));
   a.per_seg = std::max(1, (per_cta + a.segs - 1) / a.segs) * 32;
   const size_t smem = ((size_t)a.segs * a.n_local + 2 * (size_t)a.n_local) * sizeof(int);
-  static bool attr[64] = {false};
-  if (!attr[dev]) {
-    FFN_CUDA_TRY(cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      (kSortCounts + 2 * 4096) * (int)sizeof(int)));
-    attr[dev] = true;
-  }
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = pdl_allowed() ? 1 : 0;
@@ -460,6 +589,9 @@ int ffn_b200_moe_sort(size_t n_tok, size_t top_k, const int32_t *idx, int32_t ex
     (void)cudaGetLastError();
     return cuda_fail(e, "moe_sort");
   }
+  if (later)
+    FFN_LAUNCH_PDL(FFN_B200_K_ROUTE, st, "moe_sort src", src_kernel, grid_of((a.n_pairs + 255) / 256, 8), 256, 0, pos,
+                   offsets + a.n_local, src, a.n_pairs);
   return 0;
 }
 

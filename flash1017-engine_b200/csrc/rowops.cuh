@@ -8,6 +8,8 @@
 
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace ffn {
@@ -48,9 +50,17 @@ __device__ __forceinline__ void unpack(const Raw<T, VEC> &r, float (&f)[VEC]) {
 }
 template <typename T, int VEC>
 __device__ __forceinline__ Raw<T, VEC> pack(const float (&f)[VEC]) {
-  union { Raw<T, VEC> raw; T e[VEC]; } u;
+  union { Raw<T, VEC> raw; T e[VEC]; __nv_bfloat162 b[(VEC + 1) / 2]; __half2 h[(VEC + 1) / 2]; } u;
+  if constexpr (VEC % 2 == 0 && sizeof(T) == 2) {  // two roundings an instruction
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) u.e[i] = ToF32<T>::put(f[i]);
+    for (int i = 0; i < VEC / 2; ++i) {
+      if constexpr (std::is_same<T, __half>::value) u.h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      else u.b[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) u.e[i] = ToF32<T>::put(f[i]);
+  }
   return u.raw;
 }
 template <typename T, int VEC>
@@ -89,30 +99,97 @@ __device__ __forceinline__ float warp_max(float v) {
 
 // int8 codes of a row: scale = fl32(max|x| / 127), code = fl32(x / scale)
 // rounded to the nearest whole number, ties to even, within +-127.  A row of
-// zeros has scale 0 and codes 0; a row with an infinity or a NaN (max_abs not
-// finite) has scale NaN and codes 0, so that its products are NaN.
+// zeros has scale 0 and codes 0; a row with an infinity or a NaN has scale NaN
+// and codes 0, so that its products are NaN.
+//
+// The largest magnitude is taken over the bits without the sign, as unsigned
+// numbers: their order is that of the magnitudes, with infinity and then the
+// NaNs on top, so no value needs a test of its own.
+template <typename T, int VEC>
+__device__ __forceinline__ uint32_t abs_bits(const Raw<T, VEC> &r) {
+  union { Raw<T, VEC> raw; T e[VEC]; uint16_t h[sizeof(T) * VEC / 2]; uint32_t w[(sizeof(T) * VEC + 3) / 4]; } u;
+  u.raw = r;
+  if constexpr (sizeof(T) == 4) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) m = max(m, u.w[i] & 0x7fffffffu);
+    return m;
+  } else if constexpr (VEC == 1) {
+    return u.h[0] & 0x7fffu;
+  } else {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) m = __vmaxu2(m, u.w[i] & 0x7fff7fffu);
+    return max(m & 0xffffu, m >> 16);
+  }
+}
+// the magnitude with these bits of type T
+template <typename T>
+__device__ __forceinline__ float from_abs_bits(uint32_t b) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(b);
+  else {
+    union { uint16_t u; T t; } v;
+    v.u = (uint16_t)b;
+    return ToF32<T>::get(v.t);
+  }
+}
 __device__ __forceinline__ float int8_scale(float max_abs) {
   return isfinite(max_abs) ? __fdiv_rn(max_abs, 127.f) : __int_as_float(0x7fffffff);
 }
-// The quotient by a reciprocal is within 2^-22 of x / scale in relative terms
-// (127 * 2^-22 < 2^-15 in absolute ones), so only values that near a half need
-// the true division to be rounded the same way.
-__device__ __forceinline__ int int8_code(float x, float scale, float inv) {
-  const float q = x * inv;
-  float r = rintf(q);
-  if (!(fabsf(fabsf(q - r) - 0.5f) > 3.1e-5f)) r = rintf(__fdiv_rn(x, scale));
-  return (int)fminf(fmaxf(r, -127.f), 127.f);
-}
-// VEC codes at p (aligned to VEC bytes, 8 at most)
+
+// What a row's codes are computed from: x times 127 / max|x|, by the fast
+// division (2 steps, 2^-22 relative).  With the rounding of the scale that is
+// within 127 * (2^-22 + 2^-24) < 3.8e-5 of x / scale, and fl32 moves that by
+// 3.8e-6 at most; so where the product is not within 1e-4 of a half it rounds to
+// the same whole number, and next to a half the true quotients decide.  Magnitudes
+// outside the fast division's range always take those.
+struct Int8Row {
+  float max_abs, inv;
+  bool zero, divide;
+  __device__ __forceinline__ explicit Int8Row(float m) : max_abs(m) {
+    zero = !(m > 0.f && m < INFINITY);
+    divide = m < 1e-35f || m > 1e37f;
+    inv = zero || divide ? 0.f : __fdividef(127.f, m);
+  }
+  __device__ __forceinline__ float scale() const { return int8_scale(max_abs); }
+};
 template <int VEC>
-__device__ __forceinline__ void store_codes(int8_t *p, const float (&f)[VEC], float scale) {
-  // below 2^-126 the reciprocal overflows or loses bits: divide every value
-  const bool ok = scale > 0.f, tiny = scale < 1.2e-38f;
-  const float inv = ok ? (tiny ? __int_as_float(0x7fffffff) : __fdiv_rn(1.f, scale)) : 0.f;
-  union { Raw<int8_t, VEC> raw; int8_t e[VEC]; } u;
+__device__ __forceinline__ Raw<int8_t, VEC> int8_codes(const float (&f)[VEC], const Int8Row &s) {
+  // x * inv + 1.5 * 2^23, rounded once: the whole number sits in the low bits
+  constexpr float kWhole = 12582912.f;
+  uint32_t c[VEC];
+  float off = 0.f;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) u.e[i] = ok ? (int8_t)int8_code(f[i], scale, inv) : (int8_t)0;
-  *reinterpret_cast<Raw<int8_t, VEC> *>(p) = u.raw;
+  for (int i = 0; i < VEC; ++i) {
+    const float t = fmaf(f[i], s.inv, kWhole);
+    c[i] = __float_as_uint(t);
+    off = fmaxf(off, fabsf(fmaf(f[i], s.inv, kWhole - t)));
+  }
+  if (off > 0.4999f || s.divide) {
+    const float sc = s.scale();
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      c[i] = s.zero ? 0u : (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(f[i], sc)), -127.f), 127.f);
+  }
+  if (s.zero) {  // also rows that are not finite
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) c[i] = 0u;
+  }
+  union { Raw<int8_t, VEC> raw; uint32_t w[(VEC + 3) / 4]; uint8_t b[VEC]; } u;
+  if constexpr (VEC % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i)
+      u.w[i] = __byte_perm(__byte_perm(c[4 * i], c[4 * i + 1], 0x0040), __byte_perm(c[4 * i + 2], c[4 * i + 3], 0x0040), 0x5410);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) u.b[i] = (uint8_t)c[i];
+  }
+  return u.raw;
+}
+// VEC codes at p (aligned to VEC bytes)
+template <int VEC>
+__device__ __forceinline__ void store_codes(int8_t *p, const float (&f)[VEC], const Int8Row &s) {
+  *reinterpret_cast<Raw<int8_t, VEC> *>(p) = int8_codes<VEC>(f, s);
 }
 
 // Whether rows at p, ld elements of es bytes apart, can be read 16 bytes at a time.

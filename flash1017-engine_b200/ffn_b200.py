@@ -49,7 +49,8 @@ EXPORTS = [
     "ffn_b200_quantize_nvfp4x4", "ffn_b200_ep_moe_layer", "ffn_b200_set_host_cache_budget",
     "ffn_b200_topk", "ffn_b200_quantize_nvfp4_terms", "ffn_b200_fp4_pack_bytes",
     "ffn_b200_pack_nvfp4_expert",
-    "ffn_b200_quantize_int8", "ffn_b200_int8_matmul",
+    "ffn_b200_quantize_int8", "ffn_b200_int8_matmul", "ffn_b200_int8_linear_ws_bytes",
+    "ffn_b200_int8_linear",
     "ffn_b200_moe_sort", "ffn_b200_moe_permute", "ffn_b200_moe_combine", "ffn_b200_moe_combine_bwd",
     "ffn_b200_block_norm", "ffn_b200_block_norm_bwd_ws_bytes", "ffn_b200_block_norm_bwd",
 ]
@@ -200,6 +201,10 @@ def lib() -> C.CDLL:
         L.ffn_b200_quantize_int8.argtypes = [sz, sz, C.c_int32, vp, sz, C.c_int32, vp, vp, sz, vp, vp]
         L.ffn_b200_int8_matmul.argtypes = [sz, sz, sz, sz, vp, vp, sz, vp, vp, sz, vp, vp, C.c_int32,
                                            vp, sz, vp]
+        L.ffn_b200_int8_linear_ws_bytes.restype = sz
+        L.ffn_b200_int8_linear_ws_bytes.argtypes = [sz, sz, sz, vp]
+        L.ffn_b200_int8_linear.argtypes = [sz, sz, sz, sz, vp, C.c_int32, vp, sz, vp, sz, vp, vp, C.c_int32,
+                                           vp, sz, vp, sz, vp]
         L.ffn_b200_moe_sort.argtypes = [sz, sz, vp, C.c_int32, C.c_int32, vp, vp, vp, vp]
         L.ffn_b200_moe_permute.argtypes = [sz, sz, sz, vp, sz, vp, sz, vp, sz, vp, vp, vp]
         L.ffn_b200_moe_combine.argtypes = [sz, sz, sz, C.c_int32, vp, sz, sz, vp, vp, vp, sz, vp, sz,
@@ -812,76 +817,89 @@ class MoeLayer:
 # Temporaries come from torch's allocator, so calls on several streams and
 # captured graphs share none.  Nothing here takes part in autograd: the
 # gradients are calls of their own.
+#
+# One call is one or two kernel launches of a few microseconds, so the checks
+# stay lean: torch's accessors below cost 0.1 us each, current_stream() 2.
 _dts = None
+_T = _dev_now = _raw_stream = None
 
 
-def _dtype(t):
-    global _dts
-    if _dts is None:
-        torch = _torch()
-        _dts = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
-    d = _dts.get(t.dtype)
+def _setup():
+    global _T, _dts, _dev_now, _raw_stream
+    import torch
+    _dts = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
+    _dev_now, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+    lib()
+    _T = torch
+
+
+def _dtype(dtype):
+    d = _dts.get(dtype)
     if d is None:
-        raise FfnError(f"rows must be float32, bfloat16 or float16, not {t.dtype}")
+        raise FfnError(f"rows must be float32, bfloat16 or float16, not {dtype}")
     return d
 
 
-def _elsewhere(t, stream):
-    """Whether a call on t has to switch device or stream first."""
-    if not t.is_cuda:
+def _dev(t, stream):
+    """t's device index where a call on t can run as it is, -1 where the device
+    or the stream has to be switched first."""
+    if _T is None:
+        _setup()
+    d = t.get_device()
+    if d < 0:
         raise FfnError("expected CUDA tensors")
-    return stream is not None or t.device.index != _torch().cuda.current_device()
+    return d if stream is None and d == _dev_now() else -1
 
 
 def _on(t, stream):
-    torch = _torch()
     if stream is None:
-        return torch.cuda.device(t.device)
+        return _T.cuda.device(t.device)
     if stream.device != t.device:
         raise FfnError(f"the stream is on {stream.device}, the tensors on {t.device}")
-    return torch.cuda.stream(stream)
+    return _T.cuda.stream(stream)
 
 
-def _raw(t):
-    """The current stream of t's device, as the library takes it."""
-    return _torch().cuda.current_stream(t.device).cuda_stream
-
-
-def _in(t, what, like, rows=None, cols=None, dtype=None):
-    """t as rows the library reads: 2-d, contiguous inside a row."""
-    if t.dim() != 2 or (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
+def _in(t, what, dev, dtype, rows, cols):
+    """(t, row stride) as rows the library reads: 2-d, contiguous inside a row;
+    rows or cols None: any."""
+    sh = t.shape
+    if len(sh) != 2 or (rows is not None and sh[0] != rows) or (cols is not None and sh[1] != cols):
         raise FfnError(f"{what}: expected shape [{'rows' if rows is None else rows}, "
-                       f"{'cols' if cols is None else cols}], got {list(t.shape)}")
-    if t.device != like.device:
-        raise FfnError(f"{what} is on {t.device}, not on {like.device}")
-    if t.dtype != (like.dtype if dtype is None else dtype):
-        raise FfnError(f"{what}: expected {like.dtype if dtype is None else dtype}, got {t.dtype}")
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        t = t.contiguous()
-    return t
+                       f"{'cols' if cols is None else cols}], got {list(sh)}")
+    if t.get_device() != dev:
+        raise FfnError(f"{what} is on {t.device}, not on cuda:{dev}")
+    if t.dtype is not dtype:
+        raise FfnError(f"{what}: expected {dtype}, got {t.dtype}")
+    ld, one = t.stride()
+    if (one != 1 and sh[1] > 1) or (ld < sh[1] and sh[0] > 1):
+        return t.contiguous(), sh[1]
+    return t, (ld if sh[0] > 1 else max(ld, sh[1]))
 
 
-def _out(t, what, like, rows, cols, dtype=None):
-    """t as rows the library writes, or new rows."""
+def _out(t, what, dev, dtype, rows, cols):
+    """(t, row stride) as rows the library writes; t None: new rows."""
     if t is None:
-        return _torch().empty(rows, cols, dtype=like.dtype if dtype is None else dtype, device=like.device)
-    if _in(t, what, like, rows, cols, dtype) is not t:
+        return _T.empty((rows, cols), dtype=dtype, device=dev), cols
+    got, ld = _in(t, what, dev, dtype, rows, cols)
+    if got is not t:
         raise FfnError(f"{what}: output rows must be contiguous and must not overlap")
-    return t
+    return t, ld
 
 
-def _vec(t, what, like, n, dtype=None):
-    """t as n contiguous values (float32 unless said otherwise)."""
-    dtype = _torch().float32 if dtype is None else dtype
-    if t.dtype != dtype or t.device != like.device or t.numel() != n or not t.is_contiguous():
-        raise FfnError(f"{what}: expected {n} contiguous {dtype} values on {like.device}, got "
+def _vec(t, what, dev, n, dtype=None):
+    """The address of n contiguous values (float32 unless said otherwise)."""
+    if t.dtype is not (dtype or _T.float32) or t.get_device() != dev or t.numel() != n or not t.is_contiguous():
+        raise FfnError(f"{what}: expected {n} contiguous {dtype or _T.float32} values on cuda:{dev}, got "
                        f"{list(t.shape)} {t.dtype} on {t.device}")
-    return t
+    return t.data_ptr()
 
 
-def _ld(t):
-    """Row stride in elements; that of a single row may be anything."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+def _pos(pos, what, dev):
+    """(tokens, top_k, address) of a pos [tokens, top_k]."""
+    sh = pos.shape
+    if len(sh) != 2 or sh[1] == 0:
+        raise FfnError(f"{what}: pos must be int32 [tokens, top_k]")
+    return sh[0], sh[1], _vec(pos, "pos", dev, sh[0] * sh[1], _T.int32)
 
 
 def quantize_int8(x, act=ACT_NONE, codes=None, scales=None, n_rows=None, stream=None):
@@ -890,28 +908,31 @@ def quantize_int8(x, act=ACT_NONE, codes=None, scales=None, n_rows=None, stream=
     (ffn_b200_quantize_int8).  New codes are a view of rows padded to 16 bytes,
     as the int8 product takes them.  n_rows: int32 CUDA tensor of one value, the
     rows in use; the rest are left as they were."""
-    if _elsewhere(x, stream):
+    dev = _dev(x, stream)
+    if dev < 0:
         with _on(x, stream):
             return quantize_int8(x, act, codes, scales, n_rows)
-    torch = _torch()
-    dt = _dtype(x)
-    x = _in(x, "x", x)
+    dt = _dtype(x.dtype)
+    x, ld = _in(x, "x", dev, x.dtype, None, None)
     rows, cols = x.shape
     if act == ACT_SWIGLU:
         if cols % 2:
             raise FfnError("quantize_int8: ACT_SWIGLU takes an even number of columns")
         cols //= 2
     if codes is None:
-        codes = torch.empty(rows, (cols + 15) // 16 * 16, dtype=torch.int8, device=x.device)[:, :cols]
+        ldc = (cols + 15) // 16 * 16
+        codes = _T.empty((rows, ldc), dtype=_T.int8, device=dev)
+        if ldc != cols:
+            codes = codes[:, :cols]
     else:
-        codes = _out(codes, "codes", x, rows, cols, torch.int8)
-    scales = torch.empty(rows, dtype=torch.float32, device=x.device) if scales is None \
-        else _vec(scales, "scales", x, rows)
-    if n_rows is not None:
-        _vec(n_rows, "n_rows", x, 1, torch.int32)
-    check(lib().ffn_b200_quantize_int8(rows, cols, dt, x.data_ptr(), _ld(x), int(act), _ptr(n_rows),
-                                       codes.data_ptr(), _ld(codes), scales.data_ptr(), _raw(x)),
-          "quantize_int8")
+        codes, ldc = _out(codes, "codes", dev, _T.int8, rows, cols)
+    if scales is None:
+        scales = _T.empty((rows,), dtype=_T.float32, device=dev)
+    rc = _lib.ffn_b200_quantize_int8(rows, cols, dt, x.data_ptr(), ld, act,
+                                     None if n_rows is None else _vec(n_rows, "n_rows", dev, 1, _T.int32),
+                                     codes.data_ptr(), ldc, _vec(scales, "scales", dev, rows), _raw_stream(dev))
+    if rc:
+        check(rc, "quantize_int8")
     return codes, scales
 
 
@@ -922,24 +943,28 @@ class Int8Matrix:
     rows); rows that do not start on 16-byte boundaries are laid out again."""
 
     def __init__(self, w, scale, bias=None):
-        torch = _torch()
-        if w.dtype != torch.int8 or w.dim() not in (2, 3) or not w.is_cuda or 0 in w.shape:
+        dev = _dev(w, None)
+        dev = w.get_device() if dev < 0 else dev
+        sh = w.shape
+        if w.dtype is not _T.int8 or len(sh) not in (2, 3) or 0 in sh:
             raise FfnError("Int8Matrix: w must be a CUDA int8 tensor [rows, cols] or [groups, rows, cols]")
-        if w.dim() == 2:
+        st = w.stride()
+        if len(sh) == 2:
+            sh, st = (1, *sh), (sh[0] * st[0], *st)
             w = w.unsqueeze(0)
-        self.groups, self.rows, self.cols = w.shape
-        ld = w.stride(1) if self.rows > 1 else (w.stride(0) if self.groups > 1 else self.cols)
-        if self.rows == 1 and self.groups == 1:
-            ld = (self.cols + 15) // 16 * 16  # the stride of a single row is never used
-        if w.data_ptr() % 16 or ld % 16 or ld < self.cols or (self.cols > 1 and w.stride(2) != 1) or \
-                (self.groups > 1 and w.stride(0) != self.rows * ld):
-            ld = (self.cols + 15) // 16 * 16
-            wide = torch.zeros(self.groups, self.rows, ld, dtype=torch.int8, device=w.device)
-            wide[:, :, :self.cols] = w
-            w = wide[:, :, :self.cols]
-        self.w, self.ld = w, ld
-        self.scale = _vec(scale, "scale", w, self.groups * self.rows)
-        self.bias = None if bias is None else _vec(bias, "bias", w, self.groups * self.rows)
+        groups, rows, cols = sh
+        # the stride between rows, which a single row's tensor need not have
+        ld = st[1] if rows > 1 else st[0] if groups > 1 else (cols + 15) // 16 * 16
+        if ld % 16 or ld < cols or (cols > 1 and st[2] != 1) or (groups > 1 and st[0] != rows * ld) or w.data_ptr() % 16:
+            ld = (cols + 15) // 16 * 16
+            wide = _T.zeros((groups, rows, ld), dtype=_T.int8, device=w.device)
+            wide[:, :, :cols] = w
+            w = wide[:, :, :cols]
+        self.groups, self.rows, self.cols, self.w, self.ld, self.device = groups, rows, cols, w, ld, dev
+        self.scale, self.bias = scale, bias
+        _vec(scale, "scale", dev, groups * rows)
+        if bias is not None:
+            _vec(bias, "bias", dev, groups * rows)
 
     @classmethod
     def quantize(cls, w, bias=None, stream=None):
@@ -948,49 +973,52 @@ class Int8Matrix:
         if w.dim() not in (2, 3):
             raise FfnError("Int8Matrix.quantize: w must be [rows, cols] or [groups, rows, cols]")
         codes, scales = quantize_int8(w.reshape(-1, w.shape[-1]), stream=stream)
-        ld = codes.stride(0) if codes.shape[0] > 1 else (w.shape[-1] + 15) // 16 * 16
+        ld = (w.shape[-1] + 15) // 16 * 16
         codes = codes.as_strided(w.shape, ((w.shape[1] * ld, ld, 1) if w.dim() == 3 else (ld, 1)))
         return cls(codes, scales, bias)
 
     def matmul(self, x, out=None, offsets=None, dtype=None, stream=None):
         """out [tokens, rows] = x [tokens, cols] W^T, x float rows (quantised per
         token first) or their (codes, scales); in `dtype`, by default out's
-        type, x's, or float32 for codes.  Several groups: offsets int32 [groups + 1],
-        tokens offsets[g] .. offsets[g + 1] - 1 take group g, the others' rows
-        are left as they were."""
-        torch = _torch()
-        codes = x[0] if isinstance(x, (tuple, list)) else x
-        if _elsewhere(codes, stream):
-            with _on(codes, stream):
+        type, x's, or float32 for codes.  Several groups: offsets int32 [groups
+        + 1], tokens offsets[g] .. offsets[g + 1] - 1 take group g, the others'
+        rows are left as they were."""
+        floats = not isinstance(x, (tuple, list))
+        first = x if floats else x[0]
+        dev = _dev(first, stream)
+        if dev < 0:
+            with _on(first, stream):
                 return self.matmul(x, out, offsets, dtype)
+        if dev != self.device:
+            raise FfnError(f"the weights are on cuda:{self.device}, the tokens on cuda:{dev}")
+        k, m, groups = self.cols, self.rows, self.groups
         if dtype is None:
-            dtype = out.dtype if out is not None else x.dtype if codes is x else torch.float32
-        if codes is x:
-            x = _in(x, "x", self.w, None, self.cols, x.dtype)
-            n, dt = x.shape[0], _dtype(x)
-            # codes and scales in one buffer
-            ld = (self.cols + 15) // 16 * 16
-            buf = torch.empty(n * (ld + 4), dtype=torch.int8, device=x.device)
-            pc = buf.data_ptr()
-            ps, s = pc + n * ld, _raw(x)
-            check(lib().ffn_b200_quantize_int8(n, self.cols, dt, x.data_ptr(), _ld(x), ACT_NONE, None, pc, ld,
-                                               ps, s), "quantize_int8")
+            dtype = out.dtype if out is not None else x.dtype if floats else _T.float32
+        x_dtype = x.dtype if floats else _T.int8
+        first, ld = _in(first, "x", dev, x_dtype, None, k)
+        n = first.shape[0]
+        out, ldo = _out(out, "out", dev, dtype, n, m)
+        po = None if offsets is None else _vec(offsets, "offsets", dev, groups + 1, _T.int32)
+        pb = None if self.bias is None else self.bias.data_ptr()
+        if floats:
+            nb = _lib.ffn_b200_int8_linear_ws_bytes(n, k, groups, po)
+            ws = _T.empty((nb,), dtype=_T.int8, device=dev) if nb else None
+            rc = _lib.ffn_b200_int8_linear(n, m, k, groups, po, _dtype(x_dtype), first.data_ptr(), ld,
+                                           self.w.data_ptr(), self.ld, self.scale.data_ptr(), pb, _dtype(dtype),
+                                           out.data_ptr(), ldo, ws.data_ptr() if nb else None, nb, _raw_stream(dev))
         else:
-            codes, scales = x
-            codes = _in(codes, "codes", self.w, None, self.cols)
-            n, s = codes.shape[0], _raw(codes)
-            ld = codes.stride(0) if n > 1 else (self.cols + 15) // 16 * 16
-            if ld % 16 or codes.data_ptr() % 16:  # not as quantize_int8 lays them out
-                wide = torch.empty(n, (self.cols + 15) // 16 * 16, dtype=torch.int8, device=codes.device)
-                wide[:, :self.cols] = codes
-                codes, ld = wide, wide.stride(0)
-            pc, ps = codes.data_ptr(), _vec(scales, "scales", codes, n).data_ptr()
-        out = _out(out, "out", self.w, n, self.rows, dtype)
-        if offsets is not None:
-            _vec(offsets, "offsets", out, self.groups + 1, torch.int32)
-        check(lib().ffn_b200_int8_matmul(n, self.rows, self.cols, self.groups, _ptr(offsets), pc, ld, ps,
-                                         self.w.data_ptr(), self.ld, self.scale.data_ptr(), _ptr(self.bias),
-                                         _dtype(out), out.data_ptr(), _ld(out), s), "int8_matmul")
+            if n <= 1:
+                ld = (k + 15) // 16 * 16
+            if ld % 16 or first.data_ptr() % 16:  # not as quantize_int8 lays them out
+                ld = (k + 15) // 16 * 16
+                wide = _T.empty((n, ld), dtype=_T.int8, device=dev)
+                wide[:, :k] = first
+                first = wide
+            rc = _lib.ffn_b200_int8_matmul(n, m, k, groups, po, first.data_ptr(), ld, _vec(x[1], "scales", dev, n),
+                                           self.w.data_ptr(), self.ld, self.scale.data_ptr(), pb, _dtype(dtype),
+                                           out.data_ptr(), ldo, _raw_stream(dev))
+        if rc:
+            check(rc, "int8_matmul")
         return out
 
     matvec = matmul
@@ -1009,81 +1037,85 @@ def moe_sort(idx, expert_begin, expert_end, stream=None):
     the experts [expert_begin, expert_end) only: (offsets [experts + 1], pos
     [tokens, top_k] with -1 elsewhere, src [tokens * top_k] with -1 behind the
     last row), all int32 (ffn_b200_moe_sort)."""
-    if _elsewhere(idx, stream):
+    dev = _dev(idx, stream)
+    if dev < 0:
         with _on(idx, stream):
             return moe_sort(idx, expert_begin, expert_end)
-    torch = _torch()
-    if idx.dim() != 2 or idx.dtype != torch.int32 or idx.shape[1] == 0:
+    sh = idx.shape
+    if len(sh) != 2 or idx.dtype is not _T.int32 or sh[1] == 0:
         raise FfnError("moe_sort: idx must be int32 [tokens, top_k]")
-    idx = idx.contiguous()
-    n, top_k = idx.shape
     if expert_end <= expert_begin:
         raise FfnError("moe_sort: empty expert range")
-    offsets = torch.empty(expert_end - expert_begin + 1, dtype=torch.int32, device=idx.device)
-    pos = torch.empty_like(idx)
-    src = torch.empty(n * top_k, dtype=torch.int32, device=idx.device)
-    check(lib().ffn_b200_moe_sort(n, top_k, idx.data_ptr(), int(expert_begin), int(expert_end),
-                                  offsets.data_ptr(), pos.data_ptr(), src.data_ptr(), _raw(idx)), "moe_sort")
+    if not idx.is_contiguous():
+        idx = idx.contiguous()
+    offsets = _T.empty((expert_end - expert_begin + 1,), dtype=_T.int32, device=dev)
+    pos = _T.empty_like(idx)
+    src = _T.empty((sh[0] * sh[1],), dtype=_T.int32, device=dev)
+    rc = _lib.ffn_b200_moe_sort(sh[0], sh[1], idx.data_ptr(), expert_begin, expert_end, offsets.data_ptr(),
+                                pos.data_ptr(), src.data_ptr(), _raw_stream(dev))
+    if rc:
+        check(rc, "moe_sort")
     return offsets, pos, src
-
-
-def _pos(pos, what, like):
-    if pos.dim() != 2 or pos.shape[1] == 0:
-        raise FfnError(f"{what}: pos must be int32 [tokens, top_k]")
-    return _vec(pos, "pos", like, pos.numel(), _torch().int32)
 
 
 def moe_permute(x, pos, out=None, scales=None, out_scales=None, stream=None):
     """out[pos[t, k]] = x[t] for rows of any type (ffn_b200_moe_permute); new
     rows: one per pair.  With scales f32 [tokens] (int8 rows): (out,
     out_scales).  Rows that no pair names are left as they were."""
-    if _elsewhere(x, stream):
+    dev = _dev(x, stream)
+    if dev < 0:
         with _on(x, stream):
             return moe_permute(x, pos, out, scales, out_scales)
-    torch = _torch()
-    _pos(pos, "moe_permute", x)
-    n, top_k = pos.shape
-    es = x.element_size()
-    if x.dim() == 2 and x.shape[0] > 1 and x.dtype == torch.int8 and out is None and x.stride(1) == 1 and \
-            x.stride(0) > x.shape[1] and x.stride(0) == (x.shape[1] + 15) // 16 * 16:
-        # codes as quantize_int8 lays them out keep their padded rows
-        out = torch.empty(n * top_k, x.stride(0), dtype=torch.int8, device=x.device)[:, :x.shape[1]]
-    x = _in(x, "x", x, n)
-    cols = x.shape[1]
+    n, top_k, pp = _pos(pos, "moe_permute", dev)
+    x, ld = _in(x, "x", dev, x.dtype, n, None)
+    cols, es = x.shape[1], x.element_size()
     if out is None:
-        out = torch.empty(n * top_k, cols, dtype=x.dtype, device=x.device)
+        # int8 codes as quantize_int8 lays them out keep their padded rows
+        ldo = (cols + 15) // 16 * 16 if x.dtype is _T.int8 and ld % 16 == 0 else cols
+        out = _T.empty((n * top_k, ldo), dtype=x.dtype, device=dev)
+        if ldo != cols:
+            out = out[:, :cols]
+        rows = n * top_k
     else:
-        out = _out(out, "out", x, out.shape[0], cols)
+        rows = out.shape[0]
+        out, ldo = _out(out, "out", dev, x.dtype, rows, cols)
+    ps = pos_out = None
     if scales is not None:
-        _vec(scales, "scales", x, n)
-        out_scales = torch.empty(out.shape[0], dtype=torch.float32, device=x.device) if out_scales is None \
-            else _vec(out_scales, "out_scales", x, out.shape[0])
+        ps = _vec(scales, "scales", dev, n)
+        if out_scales is None:
+            out_scales = _T.empty((rows,), dtype=_T.float32, device=dev)
+        pos_out = _vec(out_scales, "out_scales", dev, rows)
     elif out_scales is not None:
         raise FfnError("moe_permute: out_scales without scales")
-    check(lib().ffn_b200_moe_permute(n, top_k, cols * es, x.data_ptr(), _ld(x) * es, pos.data_ptr(),
-                                     out.shape[0], out.data_ptr(), _ld(out) * es, _ptr(scales),
-                                     _ptr(out_scales), _raw(x)), "moe_permute")
+    rc = _lib.ffn_b200_moe_permute(n, top_k, cols * es, x.data_ptr(), ld * es, pp, rows, out.data_ptr(), ldo * es,
+                                   ps, pos_out, _raw_stream(dev))
+    if rc:
+        check(rc, "moe_permute")
     return out if scales is None else (out, out_scales)
 
 
 def moe_combine(y, pos, weight=None, residual=None, out=None, stream=None):
     """out[t] = residual[t] + sum_k weight[t, k] y[pos[t, k]] (weight f32
     [tokens, top_k] or None: 1), in f32, rounded once (ffn_b200_moe_combine)."""
-    if _elsewhere(y, stream):
+    dev = _dev(y, stream)
+    if dev < 0:
         with _on(y, stream):
             return moe_combine(y, pos, weight, residual, out)
-    dt = _dtype(y)
-    _pos(pos, "moe_combine", y)
-    y = _in(y, "y", y)
-    n, cols = pos.shape[0], y.shape[1]
-    if weight is not None:
-        _vec(weight, "weight", y, pos.numel())
+    dtype = y.dtype
+    dt = _dtype(dtype)
+    n, top_k, pp = _pos(pos, "moe_combine", dev)
+    y, ld = _in(y, "y", dev, dtype, None, None)
+    rows, cols = y.shape
+    pr, ldr = None, 0
     if residual is not None:
-        residual = _in(residual, "residual", y, n, cols)
-    out = _out(out, "out", y, n, cols)
-    check(lib().ffn_b200_moe_combine(n, pos.shape[1], cols, dt, y.data_ptr(), _ld(y), y.shape[0], pos.data_ptr(),
-                                     _ptr(weight), _ptr(residual), 0 if residual is None else _ld(residual),
-                                     out.data_ptr(), _ld(out), _raw(y)), "moe_combine")
+        residual, ldr = _in(residual, "residual", dev, dtype, n, cols)
+        pr = residual.data_ptr()
+    out, ldo = _out(out, "out", dev, dtype, n, cols)
+    rc = _lib.ffn_b200_moe_combine(n, top_k, cols, dt, y.data_ptr(), ld, rows, pp,
+                                   None if weight is None else _vec(weight, "weight", dev, n * top_k), pr, ldr,
+                                   out.data_ptr(), ldo, _raw_stream(dev))
+    if rc:
+        check(rc, "moe_combine")
     return out
 
 
@@ -1092,22 +1124,25 @@ def moe_combine_backward(dout, y, pos, weight=None, dy=None, stream=None):
     dw [tokens, top_k] f32 (ffn_b200_moe_combine_bwd).  The residual's gradient
     is dout.  A new dy has zeros in the rows that no pair names; in a given one
     they are left as they were."""
-    if _elsewhere(y, stream):
+    dev = _dev(y, stream)
+    if dev < 0:
         with _on(y, stream):
             return moe_combine_backward(dout, y, pos, weight, dy)
-    torch = _torch()
-    dt = _dtype(y)
-    _pos(pos, "moe_combine_backward", y)
-    y = _in(y, "y", y)
-    n, (rows, cols) = pos.shape[0], y.shape
-    dout = _in(dout, "dout", y, n, cols)
-    if weight is not None:
-        _vec(weight, "weight", y, pos.numel())
-    dy = torch.zeros(rows, cols, dtype=y.dtype, device=y.device) if dy is None else _out(dy, "dy", y, rows, cols)
-    dw = torch.empty(n, pos.shape[1], dtype=torch.float32, device=y.device)
-    check(lib().ffn_b200_moe_combine_bwd(n, pos.shape[1], cols, dt, dout.data_ptr(), _ld(dout), y.data_ptr(),
-                                         _ld(y), rows, pos.data_ptr(), _ptr(weight), dy.data_ptr(), _ld(dy),
-                                         dw.data_ptr(), _raw(y)), "moe_combine_bwd")
+    dtype = y.dtype
+    dt = _dtype(dtype)
+    n, top_k, pp = _pos(pos, "moe_combine_backward", dev)
+    y, ld = _in(y, "y", dev, dtype, None, None)
+    rows, cols = y.shape
+    dout, ldd = _in(dout, "dout", dev, dtype, n, cols)
+    if dy is None:
+        dy = _T.zeros((rows, cols), dtype=dtype, device=dev)
+    dy, ldy = _out(dy, "dy", dev, dtype, rows, cols)
+    dw = _T.empty((n, top_k), dtype=_T.float32, device=dev)
+    rc = _lib.ffn_b200_moe_combine_bwd(n, top_k, cols, dt, dout.data_ptr(), ldd, y.data_ptr(), ld, rows, pp,
+                                       None if weight is None else _vec(weight, "weight", dev, n * top_k),
+                                       dy.data_ptr(), ldy, dw.data_ptr(), _raw_stream(dev))
+    if rc:
+        check(rc, "moe_combine_bwd")
     return dy, dw
 
 
@@ -1126,23 +1161,22 @@ class BlockNorm:
         self.pre_w, self.post_w = pre_w, post_w
         self.alpha, self.beta, self.eps = alpha, beta, eps
 
-    def _desc(self, like, rows, cols, gate, post):
-        kind = GATE_NONE
+    def _desc(self, dev, dtype, rows, cols, gate, post):
+        kind, pg, pp, pq = GATE_NONE, None, None, None
         if gate is not None:
-            if gate.dim() == 1 and gate.shape[0] == cols:
+            sh = gate.shape
+            if len(sh) == 1 and sh[0] == cols:
                 kind = GATE_CHANNEL
-            elif gate.dim() == 2 and tuple(gate.shape) == (rows, 1):
+            elif len(sh) == 2 and sh[0] == rows and sh[1] == 1:
                 kind = GATE_TOKEN
             else:
-                raise FfnError(f"gate: expected [{cols}] or [{rows}, 1], got {list(gate.shape)}")
-            _vec(gate, "gate", like, gate.numel())
-        post_w = self.post_w if post else None
-        if post_w is not None:
-            _vec(post_w, "post_w", like, cols)
+                raise FfnError(f"gate: expected [{cols}] or [{rows}, 1], got {list(sh)}")
+            pg = _vec(gate, "gate", dev, gate.numel())
+        if post and self.post_w is not None:
+            pp = _vec(self.post_w, "post_w", dev, cols)
         if self.pre_w is not None:
-            _vec(self.pre_w, "pre_w", like, cols)
-        return BlockNormDesc(rows, cols, _dtype(like), kind, _ptr(post_w), _ptr(gate), _ptr(self.pre_w),
-                             self.alpha, self.beta, self.eps, 0)
+            pq = _vec(self.pre_w, "pre_w", dev, cols)
+        return BlockNormDesc(rows, cols, _dtype(dtype), kind, pp, pg, pq, self.alpha, self.beta, self.eps, 0)
 
     def forward(self, y, residual=None, gate=None, h=None, xn=None, codes=False, stream=None):
         """(h, xn), each a new tensor or the one given; y None: the residual
@@ -1151,76 +1185,85 @@ class BlockNorm:
         like = residual if y is None else y
         if like is None:
             raise FfnError("BlockNorm: neither y nor residual")
-        if _elsewhere(like, stream):
+        dev = _dev(like, stream)
+        if dev < 0:
             with _on(like, stream):
                 return self.forward(y, residual, gate, h, xn, codes)
-        torch = _torch()
-        if like.dim() != 2:
-            raise FfnError(f"BlockNorm: expected rows [rows, cols], got {list(like.shape)}")
-        rows, cols = like.shape
+        sh, dtype = like.shape, like.dtype
+        if len(sh) != 2:
+            raise FfnError(f"BlockNorm: expected rows [rows, cols], got {list(sh)}")
+        rows, cols = sh
         if y is None and gate is not None:
             raise FfnError("BlockNorm: a gate without y")
-        d = self._desc(like, rows, cols, gate, y is not None)
+        d = self._desc(dev, dtype, rows, cols, gate, y is not None)
+        py, ldy, pr, ldr, px, ldx, pq, ldq, ps = None, 0, None, 0, None, 0, None, 0, None
         if y is not None:
-            y = _in(y, "y", like, rows, cols)
+            y, ldy = _in(y, "y", dev, dtype, rows, cols)
+            py = y.data_ptr()
         if residual is not None:
-            residual = _in(residual, "residual", like, rows, cols)
-        h = _out(h, "h", like, rows, cols)
+            residual, ldr = _in(residual, "residual", dev, dtype, rows, cols)
+            pr = residual.data_ptr()
+        h, ldh = _out(h, "h", dev, dtype, rows, cols)
+        if xn is not None or (self.pre_w is not None and not codes):
+            xn, ldx = _out(xn, "xn", dev, dtype, rows, cols)
+            px = xn.data_ptr()
         q = sc = None
         if codes:
             if self.pre_w is None:
                 raise FfnError("BlockNorm: codes need pre_w")
-            q = torch.empty(rows, (cols + 15) // 16 * 16, dtype=torch.int8, device=like.device)[:, :cols]
-            sc = torch.empty(rows, dtype=torch.float32, device=like.device)
-        if xn is not None:
-            xn = _out(xn, "xn", like, rows, cols)
-        elif self.pre_w is not None and not codes:
-            xn = torch.empty(rows, cols, dtype=like.dtype, device=like.device)
-        check(lib().ffn_b200_block_norm(C.byref(d), _ptr(y), 0 if y is None else _ld(y), _ptr(residual),
-                                        0 if residual is None else _ld(residual), h.data_ptr(), _ld(h),
-                                        _ptr(xn), 0 if xn is None else _ld(xn), _ptr(q),
-                                        0 if q is None else _ld(q), _ptr(sc), _raw(like)), "block_norm")
+            ldq = (cols + 15) // 16 * 16
+            q = _T.empty((rows, ldq), dtype=_T.int8, device=dev)[:, :cols]
+            sc = _T.empty((rows,), dtype=_T.float32, device=dev)
+            pq, ps = q.data_ptr(), sc.data_ptr()
+        rc = _lib.ffn_b200_block_norm(C.byref(d), py, ldy, pr, ldr, h.data_ptr(), ldh, px, ldx, pq, ldq, ps,
+                                      _raw_stream(dev))
+        if rc:
+            check(rc, "block_norm")
         return (h, xn, q, sc) if codes else (h, xn)
 
     def backward(self, y, h, dh=None, dxn=None, gate=None, stream=None):
         """The gradients, from the y and h of the forward pass and the gradients
         of h (past the norm) and xn: {"dy", "dres", "dpost_w", "dgate",
         "dpre_w"}, None where there is no such input."""
-        like = next((t for t in (dxn, dh) if t is not None), None)
+        like = dh if dxn is None else dxn
         if like is None:
             raise FfnError("BlockNorm.backward: neither dh nor dxn")
-        if _elsewhere(like, stream):
+        dev = _dev(like, stream)
+        if dev < 0:
             with _on(like, stream):
                 return self.backward(y, h, dh, dxn, gate)
-        torch = _torch()
-        if like.dim() != 2:
-            raise FfnError(f"BlockNorm.backward: expected rows [rows, cols], got {list(like.shape)}")
-        rows, cols = like.shape
+        sh, dtype = like.shape, like.dtype
+        if len(sh) != 2:
+            raise FfnError(f"BlockNorm.backward: expected rows [rows, cols], got {list(sh)}")
+        rows, cols = sh
         if y is None and gate is not None:
             raise FfnError("BlockNorm.backward: a gate without y")
         if dxn is not None and (h is None or self.pre_w is None):
             raise FfnError("BlockNorm.backward: dxn needs h and pre_w")
-        d = self._desc(like, rows, cols, gate, y is not None)
-
-        def row(t, what):
-            return None if t is None else _in(t, what, like, rows, cols)
-        y, h, dh, dxn = row(y, "y"), row(h, "h"), row(dh, "dh"), row(dxn, "dxn")
+        d = self._desc(dev, dtype, rows, cols, gate, y is not None)
+        keep, at = [], []  # rows that were copied live until the call
+        for t, what in ((y, "y"), (h, "h"), (dh, "dh"), (dxn, "dxn")):
+            if t is None:
+                at += [None, 0]
+            else:
+                t, ld = _in(t, what, dev, dtype, rows, cols)
+                keep.append(t)
+                at += [t.data_ptr(), ld]
 
         def new(on, shape, dtype):
-            return torch.empty(shape, dtype=dtype, device=like.device) if on else None
-        f32 = torch.float32
-        dres = new(True, (rows, cols), like.dtype)
-        dy = new(y is not None, (rows, cols), like.dtype)
+            return _T.empty(shape, dtype=dtype, device=dev) if on else None
+        f32 = _T.float32
+        dres = new(True, (rows, cols), dtype)
+        dy = new(y is not None, (rows, cols), dtype)
         dpost = new(d.post_w is not None, (cols,), f32)
-        dgate = new(gate is not None, None if gate is None else gate.shape, f32)
+        dgate = None if gate is None else _T.empty_like(gate)
         dpre = new(dxn is not None, (cols,), f32)
-        ws = new(True, (lib().ffn_b200_block_norm_bwd_ws_bytes(C.byref(d)),), torch.uint8)
-
-        def at(t):
-            return (None, 0) if t is None else (t.data_ptr(), _ld(t))
-        check(lib().ffn_b200_block_norm_bwd(C.byref(d), *at(y), *at(h), *at(dh), *at(dxn), *at(dres), *at(dy),
-                                            _ptr(dpost), _ptr(dgate), _ptr(dpre), ws.data_ptr(), ws.numel(),
-                                            _raw(like)), "block_norm_bwd")
+        nb = _lib.ffn_b200_block_norm_bwd_ws_bytes(C.byref(d))
+        ws = new(True, (nb,), _T.uint8)
+        rc = _lib.ffn_b200_block_norm_bwd(C.byref(d), *at, dres.data_ptr(), cols, _ptr(dy), cols, _ptr(dpost),
+                                          _ptr(dgate), _ptr(dpre), ws.data_ptr(), nb, _raw_stream(dev))
+        if rc:
+            check(rc, "block_norm_bwd")
         return {"dy": dy, "dres": dres, "dpost_w": dpost, "dgate": dgate, "dpre_w": dpre}
 
 
@@ -1240,13 +1283,12 @@ class Int8Experts:
         """out[t] = residual[t] + sum_k topk_w[t, k] expert(topk_idx[t, k])(x[t]);
         x float rows [tokens, hidden], or the (codes, scales) of such rows with
         `residual` or `out` giving the type (float32 without either)."""
-        torch = _torch()
         first = x[0] if isinstance(x, (tuple, list)) else x
-        if _elsewhere(first, stream):
+        if _dev(first, stream) < 0:
             with _on(first, stream):
                 return self.forward(x, topk_idx, topk_w, residual, out)
         like = next((t for t in (x if first is x else None, residual, out) if t is not None), None)
-        dtype = torch.float32 if like is None else like.dtype
+        dtype = _T.float32 if like is None else like.dtype
         codes, scales = quantize_int8(x) if first is x else x
         offsets, pos, _ = moe_sort(topk_idx, self.expert_begin, self.expert_begin + self.gate_up.groups)
         rows = moe_permute(codes, pos, scales=scales)

@@ -340,6 +340,15 @@ FFN_B200_EXPORT int ffn_b200_int8_matmul(size_t rows, size_t n, size_t k, size_t
                                          const int8_t *x, size_t ld_x, const float *x_scales, const int8_t *w,
                                          size_t ld_w, const float *w_scales, const float *bias, int32_t dtype,
                                          void *out, size_t ld_out, void *stream);
+/* quantize_int8 of float rows x (x_dtype, k <= 16384) and int8_matmul, in one call:
+ * the same bits.  Up to 4 rows and one matrix take one launch and no workspace;
+ * else ws (16-byte aligned, int8_linear_ws_bytes) holds the codes. */
+FFN_B200_EXPORT size_t ffn_b200_int8_linear_ws_bytes(size_t rows, size_t k, size_t n_groups,
+                                                     const int32_t *offsets);
+FFN_B200_EXPORT int ffn_b200_int8_linear(size_t rows, size_t n, size_t k, size_t n_groups, const int32_t *offsets,
+                                         int32_t x_dtype, const void *x, size_t ld_x, const int8_t *w, size_t ld_w,
+                                         const float *w_scales, const float *bias, int32_t dtype, void *out,
+                                         size_t ld_out, void *ws, size_t ws_bytes, void *stream);
 
 /* --------------------------------------------- routed pairs: sort and back
  * The layer's grouping and combine (flash1017.rs:8088-8099, 8267-8326) as

@@ -3,15 +3,15 @@ and their gradient, against 64-bit restatements.
 
 Tolerances count f32 roundings: a row sum is a tree of at most 48 additions
 (32 values in a thread, 5 + 5 shuffles, and the products), so mean(v^2) is off
-by at most 50 U relative and 1 / sqrt(mean + eps) by 25 U + 3 U; every further
-product or sum adds U of its terms.  The last rounding adds half a step of
+by at most 50 U relative and its root by 25 U; rsqrtf is within 2 steps (4 U)
+and the sum with eps adds U.  Every further product or sum adds U of its terms.  The last rounding adds half a step of
 the type."""
 import pytest
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
 EPS = 1e-6
-RS = 28 * U  # relative error of 1 / sqrt(mean(v^2) + eps)
+RS = 30 * U  # relative error of 1 / sqrt(mean(v^2) + eps)
 
 ROWS_COLS = [(1, 1), (3, 7), (1, 64), (9, 65), (5, 512), (17, 513), (2, 1000), (300, 1024), (4, 1031), (33, 4096),
              (650, 5120), (1, 7168), (3, 8191), (2, 16384), (2, 16383), (2400, 96)]
@@ -154,9 +154,9 @@ def test_backward(ffn, cuda, rows, cols, dtype, gate, post):
             continue
         ref, mag = want[name]
         # every term of the chain carries at most two reciprocal roots and two
-        # row means (28 + 50 each) and a dozen products; sums over rows add at
+        # row means (30 + 50 each) and a dozen products; sums over rows add at
         # most one rounding a row
-        c = 2 * (28 + 50) + 16 + (rows if name in ("dpre_w", "dpost_w") or (name == "dgate" and gate == "channel") else 50)
+        c = 2 * (30 + 50) + 16 + (rows if name in ("dpre_w", "dpost_w") or (name == "dgate" and gate == "channel") else 50)
         err = c * U * mag
         u = half_step(torch, dt) if t.dtype == dt and name in ("dy", "dres") else U
         assert t.shape == ref.shape, name

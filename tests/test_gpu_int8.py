@@ -100,7 +100,7 @@ def test_swiglu_codes(ffn, cuda, rows, cols, dtype):
     q, s = ffn.quantize_int8(x, ffn.ACT_SWIGLU)
     gate, up = x[:, :cols].double(), x[:, cols:].double()
     v = torch.clamp(gate / (1 + torch.exp(-gate)), max=10) * up.clamp(-10, 10)
-    # expf within 2 steps, then a sum, a quotient and a product: 8 U relative
+    # expf within a step (2 U), a sum, a quotient within two (4 U), a product: 8 U
     assert ((s.double() - v.abs().amax(1) / 127).abs() <= s.double() * 10 * U).all()
     assert ((q.double() * s.double()[:, None] - v).abs() <= s.double()[:, None] * (0.5 + 127 * 20 * U) + 10 * U * v.abs()).all()
     x[0, 1] = float("nan")
