@@ -15,6 +15,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "ffn_internal.h"
 #include "rowops.cuh"
@@ -103,11 +104,17 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) quant_kernel(const QuantArg
 }
 
 // ----------------------------------------------------------------- product
-constexpr int kThreads = 192;       // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
+// Warp 0: TMA, one thread; warp 1: MMA, one thread; warps 2-5: epilogue.  The two
+// single threads set the pace, so they count stages and phases instead of
+// dividing: two divisions a stage cost more than its waits and copies together
+// (8192 x 4096 x 4096: 97 us with them, 94 us without).
+constexpr int kMmaWarp = 1;
+constexpr int kThreads = 192;
 constexpr int kM = 128;             // channels a tile
 constexpr int kKB = 128;            // K bytes (= values) a stage
 constexpr int kABytes = kM * kKB;
 constexpr int kMaxStages = 12;
+constexpr int kSplitRows = 128;      // tokens a tile, at most, where K is split over a cluster
 constexpr int kSmemMax = 224 * 1024;
 
 struct GemmArgs {
@@ -115,11 +122,12 @@ struct GemmArgs {
   const float *xs, *ws, *bias;
   void *out;
   size_t ld_out;
-  int rows, n, kt, groups;
-  int nt;      // tokens a tile, at most (16 .. 256)
-  int bx;      // rows of one token box
+  int rows, n, groups;
+  int kt, kfull;  // 128-byte blocks of K, and those that are full
+  int nt;      // tokens a tile, at most (a multiple of 16, of 32 for pairs; up to 256)
+  int sub;     // blocks of K a stage holds
   int stages;
-  int cs;      // CTAs of the cluster, each a part of K
+  int cs;      // CTAs of the cluster: each a part of K, or a pair on one tile
 };
 
 __device__ __forceinline__ uint32_t idesc_i8(int M, int N) {  // s32 += s8 * s8, both K-major
@@ -130,12 +138,91 @@ __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint3
                "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}\n"
                ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc), "r"(0), "r"(0), "r"(0), "r"(0));
 }
+// Weights and tokens: tensor maps of 3-d boxes (128 bytes of K, rows, `sub` blocks
+// of K), and of single blocks for a last one that is not full.
+struct Maps {
+  CUtensorMap w3, x3, w2, x2;
+};
+__device__ __forceinline__ void tma_3d(void *dst, const CUtensorMap *m, int y, int z, uint64_t *bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+               ::"r"(tc::sa(dst)), "l"(m), "r"(0), "r"(y), "r"(z), "r"(tc::sa(bar)) : "memory");
+}
+__device__ __forceinline__ void tma_3d_pair(void *dst, const CUtensorMap *m, int y, int z, uint32_t bar0) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];"
+               ::"r"(tc::sa(dst)), "l"(m), "r"(0), "r"(y), "r"(z), "r"(bar0) : "memory");
+}
 __device__ __forceinline__ void tma_2d(void *dst, const CUtensorMap *m, int x, int y, uint64_t *bar) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                ::"r"(tc::sa(dst)), "l"(m), "r"(x), "r"(y), "r"(tc::sa(bar)) : "memory");
 }
-__device__ __forceinline__ void tma_prefetch_l2(const CUtensorMap *m, int x, int y) {
-  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(m), "r"(x), "r"(y) : "memory");
+// Waits of this file: about two seconds, by the GPU's clock, after which `err`
+// names the wait (a poll may sleep for a while, so a count of polls says little).
+constexpr unsigned long long kWaitNs = 2000000000ull;
+__device__ __forceinline__ unsigned long long now_ns() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ bool try_bar(uint64_t *b, uint32_t par) {
+  uint32_t ok;
+  asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+               : "=r"(ok) : "r"(tc::sa(b)), "r"(par) : "memory");
+  return ok != 0;
+}
+__device__ __noinline__ bool wait_bar_long(uint64_t *b, uint32_t par, int *err, int who) {
+  unsigned long long end = 0;
+  for (int i = 0;; ++i) {
+    if (try_bar(b, par)) return true;
+    if ((i & 63) == 63) {
+      if (err && *(volatile int *)err) return false;  // another role gave up
+      const unsigned long long t = now_ns();
+      if (end == 0) end = t + kWaitNs;
+      else if (t > end) {
+        if (err) atomicCAS_block(err, 0, who);
+        return false;
+      }
+    }
+  }
+}
+__device__ __forceinline__ bool wait_bar(uint64_t *b, uint32_t par, int *err, int who) {
+  return try_bar(b, par) || wait_bar_long(b, par, err, who);
+}
+// for what completes by itself (copies, MMAs): not cut short by the others' errors
+__device__ __forceinline__ void drain_bar(uint64_t *b, uint32_t par) {
+  wait_bar(b, par, nullptr, 0);
+}
+// the same for a CTA pair: completes on the barrier of the pair's first CTA, at
+// that CTA's offset of `bar`
+__device__ __forceinline__ void tma_2d_pair(void *dst, const CUtensorMap *m, int x, int y, uint32_t bar0) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];"
+               ::"r"(tc::sa(dst)), "l"(m), "r"(x), "r"(y), "r"(bar0) : "memory");
+}
+__device__ __forceinline__ uint32_t peer_addr(const void *p, uint32_t rank) {
+  uint32_t b;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(tc::sa(p)), "r"(rank));
+  return b;
+}
+__device__ __forceinline__ void mma_i8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n"
+               ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc));
+}
+// arrive on `b` in both CTAs of the pair once this thread's MMAs have completed
+__device__ __forceinline__ void commit_pair(uint64_t *b) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               ::"r"(tc::sa(b)), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void arrive_peer(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_prefetch_l2(const CUtensorMap *m, int y, int z) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(m), "r"(0), "r"(y), "r"(z) : "memory");
+}
+// true in one lane of a converged warp
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(p));
+  return p != 0;
 }
 __device__ __forceinline__ uint32_t ctarank() {
   uint32_t r;
@@ -145,6 +232,8 @@ __device__ __forceinline__ uint32_t ctarank() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void st_peer(const void *p, uint32_t rank, int v) {
   uint32_t b;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(tc::sa(p)), "r"(rank));
@@ -158,7 +247,9 @@ struct Tile {
 // s_pre[g]: token chunks of the groups before g.  Tiles run over the groups,
 // inside a group over the channel blocks, inside a block over its token chunks,
 // so CTAs that run together share the weights' block.
+template <bool PAIR>
 __device__ __forceinline__ Tile tile_of(int t, const GemmArgs &a, const int *s_pre, const int *s_off, int ct) {
+  constexpr int kRound = PAIR ? 31 : 15;
   int lo = 0, hi = a.groups;  // the last g with s_pre[g] * ct <= t
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -167,53 +258,65 @@ __device__ __forceinline__ Tile tile_of(int t, const GemmArgs &a, const int *s_p
   // skip empty groups: s_pre is equal there, the search ends on the last of them
   const int chunks = s_pre[lo + 1] - s_pre[lo], rel = t - s_pre[lo] * ct;
   const int first = s_off[2 * lo], n = s_off[2 * lo + 1];
-  const int per = ((n + chunks - 1) / chunks + 15) & ~15;
+  const int per = ((n + chunks - 1) / chunks + kRound) & ~kRound;
   const int j = rel % chunks;
   Tile o;
   o.g = lo;
-  o.c0 = rel / chunks * kM;
+  o.c0 = rel / chunks * (PAIR ? 2 * kM : kM);
   o.r0 = first + j * per;
   o.nn = max(0, min(per, n - j * per));
   return o;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, const __grid_constant__ CUtensorMap mw,
-                                                           const __grid_constant__ CUtensorMap mx) {
+template <typename T, bool PAIR>
+__global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, const __grid_constant__ Maps maps) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], mma_done;
   __shared__ uint32_t s_tmem;
   __shared__ int s_err, s_sum[kThreads / 32];
+  __shared__ float s_xs[kSplitRows];
   uint8_t *smem = smem_raw + ((1024 - (tc::sa(smem_raw) & 1023)) & 1023);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int stage_bytes = kABytes + a.nt * kKB;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  // a stage: sub blocks of weights, then sub blocks of tokens
+  const int x_rows = PAIR ? a.nt / 2 : a.nt, x_bytes = x_rows * kKB, stage_bytes = a.sub * (kABytes + x_bytes);
   int *red = reinterpret_cast<int *>(smem + a.stages * stage_bytes);     // cs > 1: [cs][nt][128 / cs]
-  int *s_off = red + (a.cs > 1 ? kM * a.nt : 0);                          // [groups][first, count]
+  const bool split = !PAIR && a.cs > 1;
+  int *s_off = red + (split ? kM * a.nt : 0);                          // [groups][first, count]
   int *s_pre = s_off + 2 * a.groups;                                      // [groups + 1]
   // two accumulators; one where a cluster has a single tile.  At most 64 columns
   // then, so that every cluster CTA an SM can hold gets its own: clusters that
   // waited for each other's TMEM on two SMs would wait for good.
-  const int acc_cols = a.nt, tmem_cols = a.cs > 1 ? max(32, acc_cols) : 2 * acc_cols;
+  const int acc_cols = a.nt <= 16 ? 16 : 1 << (32 - __clz(a.nt - 1)), tmem_cols = split ? max(32, acc_cols) : 2 * acc_cols;
   const uint32_t rank = a.cs > 1 ? ctarank() : 0;
-  const int ct = (a.n + kM - 1) / kM;
+  const int ct = (a.n + (PAIR ? 2 : 1) * kM - 1) / ((PAIR ? 2 : 1) * kM);
 
   if (tid == 0) {
     s_err = 0;
     for (int s = 0; s < a.stages; ++s) { tc::bar_init(&full[s], 1); tc::bar_init(&empty[s], 1); }
-    for (int b = 0; b < 2; ++b) { tc::bar_init(&acc_full[b], 1); tc::bar_init(&acc_empty[b], 4); }
+    for (int b = 0; b < 2; ++b) { tc::bar_init(&acc_full[b], 1); tc::bar_init(&acc_empty[b], PAIR ? 8 : 4); }
     tc::bar_init(&mma_done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&mw) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&mx) : "memory");
+    if (a.kfull) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.w3) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.x3) : "memory");
+    }
   }
-  if (warp == 1) tc::alloc(&s_tmem, tmem_cols);
-  const int k_lo = a.kt * (int)rank / a.cs, k_hi = a.kt * ((int)rank + 1) / a.cs;
+  if (warp == kMmaWarp) {
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::sa(&s_tmem)), "r"(tmem_cols));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+      tc::alloc(&s_tmem, tmem_cols);
+    }
+  }
+  const int k_lo = split ? a.kt * (int)rank / a.cs : 0, k_hi = split ? a.kt * ((int)rank + 1) / a.cs : a.kt;
   const int tile0 = (int)(blockIdx.x / a.cs), tile_step = (int)(gridDim.x / a.cs);
-  if (!a.offsets && warp == 0 && lane < min(a.stages, k_hi - k_lo) ) {
+  if (!a.offsets && warp == 0 && lane < a.stages && k_lo + lane * a.sub < min(k_hi, a.kfull)) {
     // one group: this CTA's first weights are known before the previous kernel
     // has finished; bring them into L2 (a hint, nothing is read from it yet)
     const int chunks = (a.rows + a.nt - 1) / a.nt;
-    if (tile0 < chunks * ct) tma_prefetch_l2(&mw, (k_lo + lane) * kKB, tile0 / chunks * kM);
+    if (tile0 < chunks * ct)
+      tma_prefetch_l2(&maps.w3, PAIR ? tile0 / chunks * 2 * kM + (int)rank * kM : tile0 / chunks * kM, k_lo + lane * a.sub);
   }
   pdl_enter();
 
@@ -249,76 +352,120 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  if (a.cs > 1) cluster_sync();  // the peers' shared memory is there
+  // the peers' shared memory is there: needed before the first copy of a pair, and
+  // before the first sum leaves a part of K
+  if (PAIR) cluster_sync();
+  else if (split) cluster_arrive();
   const uint32_t tmem = s_tmem;
   const int n_tiles = s_pre[a.groups] * ct;
 
   if (warp == 0) {
     // -------------------------------------------------- TMA producer (one lane)
-    if (lane == 0) {
-      int it = 0;
+    if (elect_one()) {
+      int s = 0;
+      uint32_t ph = 0, used = 0;  // the stage, its phase, the stages ever used
       bool live = true;
       for (int t = tile0; t < n_tiles && live; t += tile_step) {
-        const Tile o = tile_of(t, a, s_pre, s_off, ct);
-        const int boxes = (o.nn + a.bx - 1) / a.bx;
-        const uint32_t bytes = kABytes + boxes * a.bx * kKB;
-        for (int k = k_lo; k < k_hi; ++k, ++it) {
-          const int s = it % a.stages;
-          if (!tc::bar_wait(&empty[s], ((it / a.stages) & 1) ^ 1, &s_err)) { live = false; break; }
-          uint8_t *st = smem + s * stage_bytes;
-          tc::bar_arrive_tx(&full[s], bytes);
-          tma_2d(st, &mw, k * kKB, o.g * a.n + o.c0, &full[s]);
-          for (int b = 0; b < boxes; ++b)
-            tma_2d(st + kABytes + b * a.bx * kKB, &mx, k * kKB, o.r0 + b * a.bx, &full[s]);
+        const Tile o = tile_of<PAIR>(t, a, s_pre, s_off, ct);
+        // a pair: each CTA brings its own 128 channels and half of the tokens, and
+        // the first CTA's barrier counts the bytes of both
+        const int row = o.r0 + (PAIR ? (int)rank * (((o.nn + 31) & ~31) / 2) : 0);
+        const int ch = o.g * a.n + o.c0 + (PAIR ? (int)rank * kM : 0);
+        for (int k = k_lo; k < k_hi; k += a.sub) {
+          if (!wait_bar(&empty[s], ph ^ 1, &s_err, 1)) { live = false; break; }
+          uint8_t *sw = smem + s * stage_bytes, *sx = sw + a.sub * kABytes;
+          const uint32_t bar0 = PAIR ? peer_addr(&full[s], 0) : 0;
+          // One copy for all blocks of a stage: a single thread issues them, and
+          // with a copy per block and per 32 tokens it was what the kernel waited
+          // for (8192 x 4096 x 4096: 145 us; one box of 128 tokens 124 us).  Blocks
+          // past the last full one read as zeros.
+          const bool tail = a.kfull < a.kt && k + a.sub > a.kfull;
+          const int n = tail ? min(a.sub, k_hi - k) : a.sub;
+          if (!PAIR || rank == 0) tc::bar_arrive_tx(&full[s], (PAIR ? 2 : 1) * n * (kABytes + x_bytes));
+          if (!tail) {
+            if constexpr (PAIR) tma_3d_pair(sw, &maps.w3, ch, k, bar0), tma_3d_pair(sx, &maps.x3, row, k, bar0);
+            else tma_3d(sw, &maps.w3, ch, k, &full[s]), tma_3d(sx, &maps.x3, row, k, &full[s]);
+          } else {
+            for (int q = 0; q < n; ++q) {
+              if constexpr (PAIR) {
+                tma_2d_pair(sw + q * kABytes, &maps.w2, (k + q) * kKB, ch, bar0);
+                tma_2d_pair(sx + q * x_bytes, &maps.x2, (k + q) * kKB, row, bar0);
+              } else {
+                tma_2d(sw + q * kABytes, &maps.w2, (k + q) * kKB, ch, &full[s]);
+                tma_2d(sx + q * x_bytes, &maps.x2, (k + q) * kKB, row, &full[s]);
+              }
+            }
+          }
+          used |= 1u << s;
+          if (++s == a.stages) s = 0, ph ^= 1;
         }
       }
-      // every copy has landed before the CTA leaves
-      for (int s = 0; s < min(a.stages, it); ++s) {
-        const int last = (it - 1 - s) / a.stages;  // the last use of stage s
-        tc::bar_wait_drain(&full[s], last & 1);
-      }
+      // Every stage has been read before the CTA leaves: its copies have landed,
+      // and no commit arrives in this shared memory any more.
+      for (int i = 0; i < a.stages; ++i)
+        if (used >> i & 1u) drain_bar(&empty[i], i < s ? ph : ph ^ 1);
     }
     __syncwarp();
-  } else if (warp == 1) {
+  } else if (warp == kMmaWarp) {
     // -------------------------------------------------- MMA issuer (one lane)
-    if (lane == 0) {
-      int it = 0, n = 0;
+    if ((!PAIR || rank == 0) && elect_one()) {
+      // Operand descriptors by addition: the start address (in 16 bytes) is their
+      // low field and stays below its 14 bits.  elect.sync rather than a lane
+      // number lets the compiler keep all of this in uniform registers, which is
+      // where the instruction wants it.
+      const uint64_t w0 = tc::desc_sw128(tc::sa(smem)), x0 = tc::desc_sw128(tc::sa(smem) + a.sub * kABytes);
+      uint64_t dw = w0, dx = x0;
+      int s = 0, n = 0;
+      uint32_t ph = 0;
       bool live = true;
       for (int t = tile0; t < n_tiles && live; t += tile_step, ++n) {
-        const Tile o = tile_of(t, a, s_pre, s_off, ct);
-        const uint32_t id = idesc_i8(kM, max(16, (o.nn + 15) & ~15));
+        const Tile o = tile_of<PAIR>(t, a, s_pre, s_off, ct);
+        const uint32_t id = PAIR ? idesc_i8(2 * kM, (o.nn + 31) & ~31) : idesc_i8(kM, (o.nn + 15) & ~15);
         const int b = n & 1;
-        if (!tc::bar_wait(&acc_empty[b], ((n >> 1) & 1) ^ 1, &s_err)) break;
+        if (!wait_bar(&acc_empty[b], ((n >> 1) & 1) ^ 1, &s_err, 2)) break;
         tc::fence_after();
-        for (int k = k_lo; k < k_hi; ++k, ++it) {
-          const int s = it % a.stages;
-          if (!tc::bar_wait(&full[s], (it / a.stages) & 1, &s_err)) { live = false; break; }
+        const uint32_t d = tmem + b * acc_cols;
+        uint32_t acc = 0;
+        for (int k = k_lo; k < k_hi; k += a.sub) {
+          const int nq = min(a.sub, k_hi - k);
+          if (!wait_bar(&full[s], ph, &s_err, 3)) { live = false; break; }
           tc::fence_after();
-          const uint32_t sa = tc::sa(smem + s * stage_bytes);
+          uint64_t qw = dw, qx = dx;
+          for (int q = 0; q < nq; ++q, qw += kABytes >> 4, qx += x_bytes >> 4) {
 #pragma unroll
-          for (int j = 0; j < kKB / 32; ++j)
-            mma_i8(tmem + b * acc_cols, tc::desc_sw128(sa + 32 * j), tc::desc_sw128(sa + kABytes + 32 * j), id,
-                   (k > k_lo || j > 0) ? 1u : 0u);
-          tc::commit(&empty[s]);
+            for (int j = 0; j < kKB / 32; ++j, acc = 1) {
+              if constexpr (PAIR) mma_i8_pair(d, qw + 2 * j, qx + 2 * j, id, acc);
+              else mma_i8(d, qw + 2 * j, qx + 2 * j, id, acc);
+            }
+          }
+          if constexpr (PAIR) commit_pair(&empty[s]);
+          else tc::commit(&empty[s]);
+          dw += stage_bytes >> 4, dx += stage_bytes >> 4;
+          if (++s == a.stages) s = 0, ph ^= 1, dw = w0, dx = x0;
         }
         if (!live) break;
-        tc::commit(&acc_full[b]);
+        if constexpr (PAIR) commit_pair(&acc_full[b]);
+        else tc::commit(&acc_full[b]);
       }
-      tc::commit(&mma_done);  // every MMA has completed before TMEM is freed
-      tc::bar_wait_drain(&mma_done, 0);
+      if constexpr (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(tc::sa(&mma_done)) : "memory");
+      else
+        tc::commit(&mma_done);  // every MMA has completed before TMEM is freed
+      drain_bar(&mma_done, 0);
     }
     __syncwarp();
   } else {
     // -------------------------------------------------- epilogue (4 warps)
     const int quarter = warp & 3, cl = quarter * 32 + lane;
     int n = 0;
+    if (split) cluster_wait();
     for (int t = tile0; t < n_tiles; t += tile_step, ++n) {
-      const Tile o = tile_of(t, a, s_pre, s_off, ct);
+      const Tile o = tile_of<PAIR>(t, a, s_pre, s_off, ct);
       const int b = n & 1;
-      const bool ok = __all_sync(0xffffffffu, tc::bar_wait(&acc_full[b], (n >> 1) & 1, &s_err));
+      const bool ok = __any_sync(0xffffffffu, lane == 0 && wait_bar(&acc_full[b], (n >> 1) & 1, &s_err, 4));
       tc::fence_after();
       const uint32_t tl = tmem + b * acc_cols + ((uint32_t)(32 * quarter) << 16);
-      if (a.cs > 1) {
+      if (split) {
         // this CTA's part of K: lane cl's sums go to the CTA that owns the channel
         const int own = kM / a.cs, dst = cl / own;
         for (int c = 0; ok && c < o.nn; c += 16) {
@@ -331,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
         }
         break;  // one tile a cluster; the sums are added up below
       }
-      const int ch = o.c0 + cl;
+      const int ch = o.c0 + (PAIR ? (int)rank * kM : 0) + cl;
       const bool on = ch < a.n;
       const float sw = on ? __ldg(a.ws + (size_t)o.g * a.n + ch) : 0.f;
       const float bias = on && a.bias ? __ldg(a.bias + (size_t)o.g * a.n + ch) : 0.f;
@@ -353,34 +500,44 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
       }
       tc::fence_before();
       __syncwarp();
-      if (lane == 0) tc::bar_arrive(&acc_empty[b]);
+      if (lane == 0) {
+        if constexpr (PAIR) arrive_peer(peer_addr(&acc_empty[b], 0));
+        else tc::bar_arrive(&acc_empty[b]);
+      }
     }
   }
-  if (a.cs > 1) {
+  if (split) {
+    if (warp <= kMmaWarp) cluster_wait();
+    // what the sums will be scaled by, loaded while they are on their way: a
+    // thread keeps one channel of this CTA's own
+    const Tile o = tile0 < n_tiles ? tile_of<PAIR>(tile0, a, s_pre, s_off, ct) : Tile{0, 0, 0, 0};
+    const int own = kM / a.cs, c = tid % own, ch = o.c0 + (int)rank * own + c, step = kThreads / own;
+    const bool on = ch < a.n && tid < step * own;
+    const float sw = on ? __ldg(a.ws + (size_t)o.g * a.n + ch) : 0.f;
+    const float bias = on && a.bias ? __ldg(a.bias + (size_t)o.g * a.n + ch) : 0.f;
+    for (int i = tid; i < o.nn; i += kThreads) s_xs[i] = __ldg(a.xs + o.r0 + i);
     __syncthreads();
     if (s_err && tid < a.cs) st_peer(&s_err, tid, 1);  // all CTAs of the cluster learn of it
     __syncwarp();
     cluster_sync();
-    if (tile0 < n_tiles) {
-      const Tile o = tile_of(tile0, a, s_pre, s_off, ct);
-      const int own = kM / a.cs;
-      for (int i = tid; i < o.nn * own; i += kThreads) {
-        const int r = i / own, c = i % own, ch = o.c0 + (int)rank * own + c;
-        if (ch >= a.n) continue;
+    if (on) {
+      T *out = reinterpret_cast<T *>(a.out) + (size_t)o.r0 * a.ld_out + ch;
+      for (int r = tid / own; r < o.nn; r += step) {
         int acc = 0;
         for (int q = 0; q < a.cs; ++q) acc += red[(q * a.nt + r) * own + c];
-        float f = product_value(acc, __ldg(a.xs + o.r0 + r), __ldg(a.ws + (size_t)o.g * a.n + ch),
-                                a.bias ? __ldg(a.bias + (size_t)o.g * a.n + ch) : 0.f);
+        float f = product_value(acc, s_xs[r], sw, bias);
         if (s_err) f = __int_as_float(0x7fffffff);
-        reinterpret_cast<T *>(a.out)[(size_t)(o.r0 + r) * a.ld_out + ch] = ToF32<T>::put(f);
+        out[(size_t)r * a.ld_out] = ToF32<T>::put(f);
       }
     }
   }
   tc::fence_before();
   __syncthreads();
-  if (warp == 1) {
+  if constexpr (PAIR) cluster_sync();  // the other CTA reads and signals in this one's shared memory
+  if (warp == kMmaWarp) {
     tc::fence_after();
-    tc::dealloc(tmem, tmem_cols);
+    if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols));
+    else tc::dealloc(tmem, tmem_cols);
   }
 }
 
@@ -544,26 +701,26 @@ EncodeFn encode_fn() {
   }();
   return fn;
 }
-// rows x k bytes at p, ld bytes apart; boxes of 128 bytes x box_rows; bytes
-// past k and rows past the end read as 0
-int encode(CUtensorMap *m, const void *p, size_t rows, size_t k, size_t ld, int box_rows) {
+// rows x k bytes at p, ld bytes apart, in boxes of 128 bytes x box_rows (x blocks,
+// over the full blocks of 128 bytes alone); rows past the end, blocks past the
+// last and bytes past k read as 0
+int encode(CUtensorMap *m, const void *p, size_t rows, size_t k, size_t ld, int box_rows, int blocks) {
   const EncodeFn fn = encode_fn();
   if (!fn) return fail(FFN_B200_ECUDA, "int8_matmul: the driver has no cuTensorMapEncodeTiled");
-  const cuuint64_t dim[2] = {k, rows}, stride[1] = {ld};
-  const cuuint32_t box[2] = {(cuuint32_t)kKB, (cuuint32_t)box_rows}, es[2] = {1, 1};
-  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(p), dim, stride, box, es,
+  const cuuint64_t dim[3] = {blocks ? (cuuint64_t)kKB : k, rows, k / kKB}, stride[2] = {ld, kKB};
+  const cuuint32_t box[3] = {(cuuint32_t)kKB, (cuuint32_t)box_rows, (cuuint32_t)blocks}, es[3] = {1, 1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, blocks ? 3 : 2, const_cast<void *>(p), dim, stride, box, es,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(FFN_B200_EINVAL, "int8_matmul: tensor map refused (code " + std::to_string((int)r) + ")");
   return 0;
 }
 
-template <typename T>
-int launch_gemm(const GemmArgs &a, int grid, size_t smem, const CUtensorMap &mw, const CUtensorMap &mx, int dev,
-                cudaStream_t st) {
+template <typename T, bool PAIR>
+int launch_gemm(const GemmArgs &a, int grid, size_t smem, const Maps &maps, int dev, cudaStream_t st) {
   static bool attr[64] = {false};
   if (!attr[dev]) {
-    FFN_CUDA_TRY(cudaFuncSetAttribute(gemm_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax));
+    FFN_CUDA_TRY(cudaFuncSetAttribute(gemm_kernel<T, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax));
     attr[dev] = true;
   }
   cudaLaunchAttribute at[2];
@@ -580,7 +737,7 @@ int launch_gemm(const GemmArgs &a, int grid, size_t smem, const CUtensorMap &mw,
   cfg.attrs = at;
   cfg.numAttrs = a.cs > 1 ? 2 : 1;
   prof_begin(FFN_B200_K_INT8_GEMM, st);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_kernel<T>, a, mw, mx);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_kernel<T, PAIR>, a, maps);
   prof_end(FFN_B200_K_INT8_GEMM, st);
   note_launch();
   if (e != cudaSuccess) {
@@ -593,9 +750,10 @@ int launch_gemm(const GemmArgs &a, int grid, size_t smem, const CUtensorMap &mw,
 // Checks a product and lays out its launch (p.grid 0: nothing to do).
 struct GemmPlan {
   GemmArgs a;
-  CUtensorMap mw, mx;
+  Maps maps;
   size_t smem;
   int grid, dev;
+  bool pair;  // CTA pairs on tiles of 256 channels
 };
 int plan_gemm(GemmPlan &p, size_t rows, size_t n, size_t k, size_t n_groups, const int32_t *offsets, const int8_t *x,
               size_t ld_x, const float *x_scales, const int8_t *w, size_t ld_w, const float *w_scales, const float *bias,
@@ -624,35 +782,88 @@ int plan_gemm(GemmPlan &p, size_t rows, size_t n, size_t k, size_t n_groups, con
   a.out = out, a.ld_out = ld_out;
   a.rows = (int)rows, a.n = (int)n, a.groups = (int)n_groups;
   a.kt = (int)((k + kKB - 1) / kKB);
-  // tokens a tile: the smallest that holds an average group (a third on top for
-  // uneven ones)
-  const size_t avg = offsets ? (rows + n_groups - 1) / n_groups * 4 / 3 : rows;
-  a.nt = avg <= 16 ? 16 : avg <= 32 ? 32 : avg <= 64 ? 64 : avg <= 128 ? 128 : 256;
-  a.bx = std::min(a.nt, 64);
-  const long long ct = (long long)((n + kM - 1) / kM);
+  a.kfull = (int)(k / kKB);
+  const long long ct1 = (long long)((n + kM - 1) / kM), ct2 = (long long)((n + 2 * kM - 1) / (2 * kM));
+  a.cs = 1;
+  if (offsets) {
+    // Groups: bound by the weights' bytes, so one chunk should hold a group: the
+    // average and three deviations of an even routing (48 experts, 128 rows each:
+    // 89.5 us with 192 rows a tile, 92.9 with 160, 90.6 with 256; 8 rows each: 122
+    // us with 32 rows, 125 with 16).
+    const double avg = (double)rows / n_groups, want = avg + 3 * sqrt(avg);
+    a.nt = want <= 16 ? 16 : want >= 256 ? 256 : ((int)ceil(want) + 31) / 32 * 32;
+    p.pair = a.nt > 128 && n > (size_t)kM;
+    if (!p.pair) a.nt = std::min(a.nt, 128);
+  } else {
+    // One matrix: the cheapest of the tiles by waves x blocks of K x time a block,
+    // in us as measured at 4096 x 4096 (single CTA 0.10 + 0.0029 a token, pair 0.12
+    // + 0.00135; 77 rows x 5120 x 2304: 9.5 us with 16 rows a tile, 11.5 with 32,
+    // 12.9 with 48; 512 x 4096 x 4096: pairs of 128 rows 14.1, single 128 rows
+    // 18.8).  K split over a cluster costs 3.5 us more than it saves in blocks, and
+    // pays for few channels and a long K (16 x 8192 x 1024: 7.9 us, 11.9 without).
+    double best = 1e300;
+    auto consider = [&](int nt, bool pair, int cs) {
+      const int chunks = (int)((rows + nt - 1) / nt), round = pair ? 32 : 16;
+      const double per = (double)((rows + chunks - 1) / chunks + round - 1) / round * round;
+      const double tiles = (double)chunks * (pair ? ct2 : ct1);
+      const double waves = cs > 1 ? 1 : ceil(tiles / (pair ? sms / 2 : sms));
+      double us = waves * ceil((double)a.kt / cs) * (pair ? 0.12 + 0.00135 * per : 0.10 + 0.0029 * per);
+      if (cs > 1) us += 3.5 + 0.02 * per;
+      if (us < best) best = us, a.nt = nt, p.pair = pair, a.cs = cs;
+    };
+    for (int nt : {16, 32, 48, 64, 96, 128}) {
+      consider(nt, false, 1);
+      // clusters that are sure to be resident at once
+      const long long tiles = ct1 * (long long)((rows + nt - 1) / nt);
+      for (int cs = 2; cs <= 8 && tiles * cs <= sms * 3 / 4 && a.kt >= 4 * cs; cs *= 2) consider(nt, false, cs);
+      if ((size_t)nt >= rows) break;
+    }
+    if (n > (size_t)kM && rows > 64)
+      for (int nt : {128, 160, 192, 224, 256}) consider(nt, true, 1);
+  }
+  if (p.pair) a.cs = 2;
+  const long long ct = p.pair ? ct2 : ct1;
   // tiles at most: each group may end in a partial chunk
   const long long chunks = offsets ? std::min<long long>(rows, rows / a.nt + n_groups) : (rows + a.nt - 1) / a.nt;
   const long long tiles = ct * chunks;
   // (the kernel's tile numbers stay in 32 bits even where offsets are not ascending)
   if ((double)(rows / a.nt + 1) * (double)n_groups * (double)ct > 2147483647.0) return fail(FFN_B200_EINVAL, "int8_matmul: too many tiles");
-  // few tiles: K split over a cluster
-  a.cs = 1;
-  if (a.nt <= 64)
-    while (a.cs < 8 && tiles * a.cs * 2 <= sms && a.kt >= 4 * a.cs) a.cs *= 2;
-  const size_t tail = (a.cs > 1 ? (size_t)kM * a.nt * 4 : 0) + (3 * n_groups + 1) * sizeof(int);
-  const size_t stage = (size_t)kABytes + (size_t)a.nt * kKB;
-  a.stages = (int)std::min<size_t>({(kSmemMax - 1024 - tail) / stage, (size_t)kMaxStages, (size_t)std::max(2, a.kt)});
+  const size_t tail = (!p.pair && a.cs > 1 ? (size_t)kM * a.nt * 4 : 0) + (3 * n_groups + 1) * sizeof(int);
+  const size_t block = (size_t)kABytes + (size_t)(p.pair ? a.nt / 2 : a.nt) * kKB, room = kSmemMax - 1024 - tail;
+  // as many blocks a stage, up to 4, as leave three stages (four for pairs): each
+  // costs its threads a wait and a commit (64 blocks, 16 rows: 12.1 us with 4 a
+  // stage, 18.9 with 1), and DRAM likes the rows' bytes together
+  a.sub = 4;
+  while (a.sub > 1 && ((p.pair ? 4 : 3) * a.sub * block > room || a.kt < 2 * a.sub * (p.pair ? 1 : a.cs))) --a.sub;
+  const size_t stage = a.sub * block;
+  a.stages = (int)std::min<size_t>({room / stage, (size_t)kMaxStages, (size_t)std::max(2, a.kt)});
   if (a.stages < 2) return fail(FFN_B200_EUNSUP, "int8_matmul: too many groups for shared memory");
   p.smem = 1024 + a.stages * stage + tail;
-  if (int rc = encode(&p.mw, w, n_groups * n, k, ld_w, kM)) return rc;
-  if (int rc = encode(&p.mx, x, rows, k, ld_x, a.bx)) return rc;
-  p.grid = a.cs > 1 ? (int)tiles * a.cs : (int)std::min<long long>(tiles, sms);
+  // A pair waits for the TMEM of both its SMs at once.  It takes so much shared
+  // memory that no CTA of a K-splitting cluster fits beside it, so the two never
+  // wait for each other's columns.
+  if (p.pair) p.smem = std::max<size_t>(p.smem, 196 * 1024);
+  const int xr = p.pair ? a.nt / 2 : a.nt;
+  if (a.kfull) {
+    if (int rc = encode(&p.maps.w3, w, n_groups * n, k, ld_w, kM, a.sub)) return rc;
+    if (int rc = encode(&p.maps.x3, x, rows, k, ld_x, xr, a.sub)) return rc;
+  }
+  if (a.kfull < a.kt) {
+    if (int rc = encode(&p.maps.w2, w, n_groups * n, k, ld_w, kM, 0)) return rc;
+    if (int rc = encode(&p.maps.x2, x, rows, k, ld_x, xr, 0)) return rc;
+  }
+  p.grid = p.pair ? 2 * (int)std::min<long long>(tiles, sms / 2) : a.cs > 1 ? (int)tiles * a.cs : (int)std::min<long long>(tiles, sms);
   return 0;
 }
+template <typename T>
+int run_gemm_as(const GemmPlan &p, cudaStream_t st) {
+  return p.pair ? launch_gemm<T, true>(p.a, p.grid, p.smem, p.maps, p.dev, st)
+                : launch_gemm<T, false>(p.a, p.grid, p.smem, p.maps, p.dev, st);
+}
 int run_gemm(const GemmPlan &p, int32_t dtype, cudaStream_t st) {
-  if (dtype == FFN_B200_DT_F32) return launch_gemm<float>(p.a, p.grid, p.smem, p.mw, p.mx, p.dev, st);
-  if (dtype == FFN_B200_DT_BF16) return launch_gemm<__nv_bfloat16>(p.a, p.grid, p.smem, p.mw, p.mx, p.dev, st);
-  return launch_gemm<__half>(p.a, p.grid, p.smem, p.mw, p.mx, p.dev, st);
+  if (dtype == FFN_B200_DT_F32) return run_gemm_as<float>(p, st);
+  if (dtype == FFN_B200_DT_BF16) return run_gemm_as<__nv_bfloat16>(p, st);
+  return run_gemm_as<__half>(p, st);
 }
 
 template <typename T, int VEC, bool SWIGLU>
@@ -712,7 +923,7 @@ int ffn_b200_int8_matmul(size_t rows, size_t n, size_t k, size_t n_groups, const
                          size_t ld_x, const float *x_scales, const int8_t *w, size_t ld_w, const float *w_scales,
                          const float *bias, int32_t dtype, void *out, size_t ld_out, void *stream) {
   using namespace ffn::i8;
-  GemmPlan p;
+  GemmPlan p{};
   if (int rc = plan_gemm(p, rows, n, k, n_groups, offsets, x, ld_x, x_scales, w, ld_w, w_scales, bias, dtype, out, ld_out))
     return rc;
   return p.grid ? run_gemm(p, dtype, (cudaStream_t)stream) : 0;
@@ -736,7 +947,7 @@ int ffn_b200_int8_linear(size_t rows, size_t n, size_t k, size_t n_groups, const
     if (ws_bytes < rows * (ld + sizeof(float))) return fail(FFN_B200_ENOSPC, "int8_linear: workspace too small");
     int8_t *codes = (int8_t *)ws;
     float *scales = (float *)(codes + rows * ld);
-    GemmPlan p;
+    GemmPlan p{};
     if (int rc = plan_gemm(p, rows, n, k, n_groups, offsets, codes, ld, scales, w, ld_w, w_scales, bias, dtype, out, ld_out))
       return rc;
     // rows behind the last group's are in no product: not quantised either
