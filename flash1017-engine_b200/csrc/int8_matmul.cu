@@ -124,10 +124,10 @@ struct GemmArgs {
   size_t ld_out;
   int rows, n, groups;
   int kt, kfull;  // 128-byte blocks of K, and those that are full
-  int nt;      // tokens a tile, at most (a multiple of 16, of 32 for pairs; up to 256)
+  int nt;      // tokens a tile, at most (a multiple of 16 up to 256)
   int sub;     // blocks of K a stage holds
   int stages;
-  int cs;      // CTAs of the cluster: each a part of K, or a pair on one tile
+  int cs;      // CTAs of the cluster, each a part of K
 };
 
 __device__ __forceinline__ uint32_t idesc_i8(int M, int N) {  // s32 += s8 * s8, both K-major
@@ -147,16 +147,12 @@ __device__ __forceinline__ void tma_3d(void *dst, const CUtensorMap *m, int y, i
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
                ::"r"(tc::sa(dst)), "l"(m), "r"(0), "r"(y), "r"(z), "r"(tc::sa(bar)) : "memory");
 }
-__device__ __forceinline__ void tma_3d_pair(void *dst, const CUtensorMap *m, int y, int z, uint32_t bar0) {
-  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];"
-               ::"r"(tc::sa(dst)), "l"(m), "r"(0), "r"(y), "r"(z), "r"(bar0) : "memory");
-}
 __device__ __forceinline__ void tma_2d(void *dst, const CUtensorMap *m, int x, int y, uint64_t *bar) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                ::"r"(tc::sa(dst)), "l"(m), "r"(x), "r"(y), "r"(tc::sa(bar)) : "memory");
 }
 // Waits of this file: about two seconds, by the GPU's clock, after which `err`
-// names the wait (a poll may sleep for a while, so a count of polls says little).
+// names the wait.
 constexpr unsigned long long kWaitNs = 2000000000ull;
 __device__ __forceinline__ unsigned long long now_ns() {
   unsigned long long t;
@@ -172,7 +168,11 @@ __device__ __forceinline__ bool try_bar(uint64_t *b, uint32_t par) {
 __device__ __noinline__ bool wait_bar_long(uint64_t *b, uint32_t par, int *err, int who) {
   unsigned long long end = 0;
   for (int i = 0;; ++i) {
-    if (try_bar(b, par)) return true;
+    // test_wait returns at once (try_wait may sleep for as long as the hardware likes)
+    uint32_t ok;
+    asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                 : "=r"(ok) : "r"(tc::sa(b)), "r"(par) : "memory");
+    if (ok) return true;
     if ((i & 63) == 63) {
       if (err && *(volatile int *)err) return false;  // another role gave up
       const unsigned long long t = now_ns();
@@ -190,30 +190,6 @@ __device__ __forceinline__ bool wait_bar(uint64_t *b, uint32_t par, int *err, in
 // for what completes by itself (copies, MMAs): not cut short by the others' errors
 __device__ __forceinline__ void drain_bar(uint64_t *b, uint32_t par) {
   wait_bar(b, par, nullptr, 0);
-}
-// the same for a CTA pair: completes on the barrier of the pair's first CTA, at
-// that CTA's offset of `bar`
-__device__ __forceinline__ void tma_2d_pair(void *dst, const CUtensorMap *m, int x, int y, uint32_t bar0) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];"
-               ::"r"(tc::sa(dst)), "l"(m), "r"(x), "r"(y), "r"(bar0) : "memory");
-}
-__device__ __forceinline__ uint32_t peer_addr(const void *p, uint32_t rank) {
-  uint32_t b;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(tc::sa(p)), "r"(rank));
-  return b;
-}
-__device__ __forceinline__ void mma_i8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-               "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n"
-               ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc));
-}
-// arrive on `b` in both CTAs of the pair once this thread's MMAs have completed
-__device__ __forceinline__ void commit_pair(uint64_t *b) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-               ::"r"(tc::sa(b)), "h"((uint16_t)3) : "memory");
-}
-__device__ __forceinline__ void arrive_peer(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void tma_prefetch_l2(const CUtensorMap *m, int y, int z) {
   asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(m), "r"(0), "r"(y), "r"(z) : "memory");
@@ -247,9 +223,7 @@ struct Tile {
 // s_pre[g]: token chunks of the groups before g.  Tiles run over the groups,
 // inside a group over the channel blocks, inside a block over its token chunks,
 // so CTAs that run together share the weights' block.
-template <bool PAIR>
 __device__ __forceinline__ Tile tile_of(int t, const GemmArgs &a, const int *s_pre, const int *s_off, int ct) {
-  constexpr int kRound = PAIR ? 31 : 15;
   int lo = 0, hi = a.groups;  // the last g with s_pre[g] * ct <= t
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -258,17 +232,17 @@ __device__ __forceinline__ Tile tile_of(int t, const GemmArgs &a, const int *s_p
   // skip empty groups: s_pre is equal there, the search ends on the last of them
   const int chunks = s_pre[lo + 1] - s_pre[lo], rel = t - s_pre[lo] * ct;
   const int first = s_off[2 * lo], n = s_off[2 * lo + 1];
-  const int per = ((n + chunks - 1) / chunks + kRound) & ~kRound;
+  const int per = ((n + chunks - 1) / chunks + 15) & ~15;
   const int j = rel % chunks;
   Tile o;
   o.g = lo;
-  o.c0 = rel / chunks * (PAIR ? 2 * kM : kM);
+  o.c0 = rel / chunks * kM;
   o.r0 = first + j * per;
   o.nn = max(0, min(per, n - j * per));
   return o;
 }
 
-template <typename T, bool PAIR>
+template <typename T>
 __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, const __grid_constant__ Maps maps) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], mma_done;
@@ -278,9 +252,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
   uint8_t *smem = smem_raw + ((1024 - (tc::sa(smem_raw) & 1023)) & 1023);
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   // a stage: sub blocks of weights, then sub blocks of tokens
-  const int x_rows = PAIR ? a.nt / 2 : a.nt, x_bytes = x_rows * kKB, stage_bytes = a.sub * (kABytes + x_bytes);
+  const int x_bytes = a.nt * kKB, stage_bytes = a.sub * (kABytes + x_bytes);
   int *red = reinterpret_cast<int *>(smem + a.stages * stage_bytes);     // cs > 1: [cs][nt][128 / cs]
-  const bool split = !PAIR && a.cs > 1;
+  const bool split = a.cs > 1;
   int *s_off = red + (split ? kM * a.nt : 0);                          // [groups][first, count]
   int *s_pre = s_off + 2 * a.groups;                                      // [groups + 1]
   // two accumulators; one where a cluster has a single tile.  At most 64 columns
@@ -288,12 +262,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
   // waited for each other's TMEM on two SMs would wait for good.
   const int acc_cols = a.nt <= 16 ? 16 : 1 << (32 - __clz(a.nt - 1)), tmem_cols = split ? max(32, acc_cols) : 2 * acc_cols;
   const uint32_t rank = a.cs > 1 ? ctarank() : 0;
-  const int ct = (a.n + (PAIR ? 2 : 1) * kM - 1) / ((PAIR ? 2 : 1) * kM);
+  const int ct = (a.n + kM - 1) / kM;
 
   if (tid == 0) {
     s_err = 0;
     for (int s = 0; s < a.stages; ++s) { tc::bar_init(&full[s], 1); tc::bar_init(&empty[s], 1); }
-    for (int b = 0; b < 2; ++b) { tc::bar_init(&acc_full[b], 1); tc::bar_init(&acc_empty[b], PAIR ? 8 : 4); }
+    for (int b = 0; b < 2; ++b) { tc::bar_init(&acc_full[b], 1); tc::bar_init(&acc_empty[b], 4); }
     tc::bar_init(&mma_done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (a.kfull) {
@@ -301,14 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
       asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.x3) : "memory");
     }
   }
-  if (warp == kMmaWarp) {
-    if constexpr (PAIR) {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::sa(&s_tmem)), "r"(tmem_cols));
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
-    } else {
-      tc::alloc(&s_tmem, tmem_cols);
-    }
-  }
+  if (warp == kMmaWarp) tc::alloc(&s_tmem, tmem_cols);
   const int k_lo = split ? a.kt * (int)rank / a.cs : 0, k_hi = split ? a.kt * ((int)rank + 1) / a.cs : a.kt;
   const int tile0 = (int)(blockIdx.x / a.cs), tile_step = (int)(gridDim.x / a.cs);
   if (!a.offsets && warp == 0 && lane < a.stages && k_lo + lane * a.sub < min(k_hi, a.kfull)) {
@@ -316,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
     // has finished; bring them into L2 (a hint, nothing is read from it yet)
     const int chunks = (a.rows + a.nt - 1) / a.nt;
     if (tile0 < chunks * ct)
-      tma_prefetch_l2(&maps.w3, PAIR ? tile0 / chunks * 2 * kM + (int)rank * kM : tile0 / chunks * kM, k_lo + lane * a.sub);
+      tma_prefetch_l2(&maps.w3, tile0 / chunks * kM, k_lo + lane * a.sub);
   }
   pdl_enter();
 
@@ -352,10 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  // the peers' shared memory is there: needed before the first copy of a pair, and
-  // before the first sum leaves a part of K
-  if (PAIR) cluster_sync();
-  else if (split) cluster_arrive();
+  if (split) cluster_arrive();  // waited for before the first sum goes to a peer
   const uint32_t tmem = s_tmem;
   const int n_tiles = s_pre[a.groups] * ct;
 
@@ -366,34 +330,25 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
       uint32_t ph = 0, used = 0;  // the stage, its phase, the stages ever used
       bool live = true;
       for (int t = tile0; t < n_tiles && live; t += tile_step) {
-        const Tile o = tile_of<PAIR>(t, a, s_pre, s_off, ct);
-        // a pair: each CTA brings its own 128 channels and half of the tokens, and
-        // the first CTA's barrier counts the bytes of both
-        const int row = o.r0 + (PAIR ? (int)rank * (((o.nn + 31) & ~31) / 2) : 0);
-        const int ch = o.g * a.n + o.c0 + (PAIR ? (int)rank * kM : 0);
+        const Tile o = tile_of(t, a, s_pre, s_off, ct);
+        const int ch = o.g * a.n + o.c0;
         for (int k = k_lo; k < k_hi; k += a.sub) {
           if (!wait_bar(&empty[s], ph ^ 1, &s_err, 1)) { live = false; break; }
           uint8_t *sw = smem + s * stage_bytes, *sx = sw + a.sub * kABytes;
-          const uint32_t bar0 = PAIR ? peer_addr(&full[s], 0) : 0;
           // One copy for all blocks of a stage: a single thread issues them, and
           // with a copy per block and per 32 tokens it was what the kernel waited
           // for (8192 x 4096 x 4096: 145 us; one box of 128 tokens 124 us).  Blocks
           // past the last full one read as zeros.
           const bool tail = a.kfull < a.kt && k + a.sub > a.kfull;
           const int n = tail ? min(a.sub, k_hi - k) : a.sub;
-          if (!PAIR || rank == 0) tc::bar_arrive_tx(&full[s], (PAIR ? 2 : 1) * n * (kABytes + x_bytes));
+          tc::bar_arrive_tx(&full[s], n * (kABytes + x_bytes));
           if (!tail) {
-            if constexpr (PAIR) tma_3d_pair(sw, &maps.w3, ch, k, bar0), tma_3d_pair(sx, &maps.x3, row, k, bar0);
-            else tma_3d(sw, &maps.w3, ch, k, &full[s]), tma_3d(sx, &maps.x3, row, k, &full[s]);
+            tma_3d(sw, &maps.w3, ch, k, &full[s]);
+            tma_3d(sx, &maps.x3, o.r0, k, &full[s]);
           } else {
             for (int q = 0; q < n; ++q) {
-              if constexpr (PAIR) {
-                tma_2d_pair(sw + q * kABytes, &maps.w2, (k + q) * kKB, ch, bar0);
-                tma_2d_pair(sx + q * x_bytes, &maps.x2, (k + q) * kKB, row, bar0);
-              } else {
-                tma_2d(sw + q * kABytes, &maps.w2, (k + q) * kKB, ch, &full[s]);
-                tma_2d(sx + q * x_bytes, &maps.x2, (k + q) * kKB, row, &full[s]);
-              }
+              tma_2d(sw + q * kABytes, &maps.w2, (k + q) * kKB, ch, &full[s]);
+              tma_2d(sx + q * x_bytes, &maps.x2, (k + q) * kKB, o.r0, &full[s]);
             }
           }
           used |= 1u << s;
@@ -408,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
     __syncwarp();
   } else if (warp == kMmaWarp) {
     // -------------------------------------------------- MMA issuer (one lane)
-    if ((!PAIR || rank == 0) && elect_one()) {
+    if (elect_one()) {
       // Operand descriptors by addition: the start address (in 16 bytes) is their
       // low field and stays below its 14 bits.  elect.sync rather than a lane
       // number lets the compiler keep all of this in uniform registers, which is
@@ -419,8 +374,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
       uint32_t ph = 0;
       bool live = true;
       for (int t = tile0; t < n_tiles && live; t += tile_step, ++n) {
-        const Tile o = tile_of<PAIR>(t, a, s_pre, s_off, ct);
-        const uint32_t id = PAIR ? idesc_i8(2 * kM, (o.nn + 31) & ~31) : idesc_i8(kM, (o.nn + 15) & ~15);
+        const Tile o = tile_of(t, a, s_pre, s_off, ct);
+        const uint32_t id = idesc_i8(kM, (o.nn + 15) & ~15);
         const int b = n & 1;
         if (!wait_bar(&acc_empty[b], ((n >> 1) & 1) ^ 1, &s_err, 2)) break;
         tc::fence_after();
@@ -433,24 +388,16 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
           uint64_t qw = dw, qx = dx;
           for (int q = 0; q < nq; ++q, qw += kABytes >> 4, qx += x_bytes >> 4) {
 #pragma unroll
-            for (int j = 0; j < kKB / 32; ++j, acc = 1) {
-              if constexpr (PAIR) mma_i8_pair(d, qw + 2 * j, qx + 2 * j, id, acc);
-              else mma_i8(d, qw + 2 * j, qx + 2 * j, id, acc);
-            }
+            for (int j = 0; j < kKB / 32; ++j, acc = 1) mma_i8(d, qw + 2 * j, qx + 2 * j, id, acc);
           }
-          if constexpr (PAIR) commit_pair(&empty[s]);
-          else tc::commit(&empty[s]);
+          tc::commit(&empty[s]);
           dw += stage_bytes >> 4, dx += stage_bytes >> 4;
           if (++s == a.stages) s = 0, ph ^= 1, dw = w0, dx = x0;
         }
         if (!live) break;
-        if constexpr (PAIR) commit_pair(&acc_full[b]);
-        else tc::commit(&acc_full[b]);
+        tc::commit(&acc_full[b]);
       }
-      if constexpr (PAIR)
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(tc::sa(&mma_done)) : "memory");
-      else
-        tc::commit(&mma_done);  // every MMA has completed before TMEM is freed
+      tc::commit(&mma_done);  // every MMA has completed before TMEM is freed
       drain_bar(&mma_done, 0);
     }
     __syncwarp();
@@ -460,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
     int n = 0;
     if (split) cluster_wait();
     for (int t = tile0; t < n_tiles; t += tile_step, ++n) {
-      const Tile o = tile_of<PAIR>(t, a, s_pre, s_off, ct);
+      const Tile o = tile_of(t, a, s_pre, s_off, ct);
       const int b = n & 1;
       const bool ok = __any_sync(0xffffffffu, lane == 0 && wait_bar(&acc_full[b], (n >> 1) & 1, &s_err, 4));
       tc::fence_after();
@@ -478,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
         }
         break;  // one tile a cluster; the sums are added up below
       }
-      const int ch = o.c0 + (PAIR ? (int)rank * kM : 0) + cl;
+      const int ch = o.c0 + cl;
       const bool on = ch < a.n;
       const float sw = on ? __ldg(a.ws + (size_t)o.g * a.n + ch) : 0.f;
       const float bias = on && a.bias ? __ldg(a.bias + (size_t)o.g * a.n + ch) : 0.f;
@@ -500,17 +447,14 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
       }
       tc::fence_before();
       __syncwarp();
-      if (lane == 0) {
-        if constexpr (PAIR) arrive_peer(peer_addr(&acc_empty[b], 0));
-        else tc::bar_arrive(&acc_empty[b]);
-      }
+      if (lane == 0) tc::bar_arrive(&acc_empty[b]);
     }
   }
   if (split) {
     if (warp <= kMmaWarp) cluster_wait();
     // what the sums will be scaled by, loaded while they are on their way: a
     // thread keeps one channel of this CTA's own
-    const Tile o = tile0 < n_tiles ? tile_of<PAIR>(tile0, a, s_pre, s_off, ct) : Tile{0, 0, 0, 0};
+    const Tile o = tile0 < n_tiles ? tile_of(tile0, a, s_pre, s_off, ct) : Tile{0, 0, 0, 0};
     const int own = kM / a.cs, c = tid % own, ch = o.c0 + (int)rank * own + c, step = kThreads / own;
     const bool on = ch < a.n && tid < step * own;
     const float sw = on ? __ldg(a.ws + (size_t)o.g * a.n + ch) : 0.f;
@@ -533,11 +477,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
   }
   tc::fence_before();
   __syncthreads();
-  if constexpr (PAIR) cluster_sync();  // the other CTA reads and signals in this one's shared memory
   if (warp == kMmaWarp) {
     tc::fence_after();
-    if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols));
-    else tc::dealloc(tmem, tmem_cols);
+    tc::dealloc(tmem, tmem_cols);
   }
 }
 
@@ -716,11 +658,11 @@ int encode(CUtensorMap *m, const void *p, size_t rows, size_t k, size_t ld, int 
   return 0;
 }
 
-template <typename T, bool PAIR>
+template <typename T>
 int launch_gemm(const GemmArgs &a, int grid, size_t smem, const Maps &maps, int dev, cudaStream_t st) {
   static bool attr[64] = {false};
   if (!attr[dev]) {
-    FFN_CUDA_TRY(cudaFuncSetAttribute(gemm_kernel<T, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax));
+    FFN_CUDA_TRY(cudaFuncSetAttribute(gemm_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax));
     attr[dev] = true;
   }
   cudaLaunchAttribute at[2];
@@ -737,7 +679,7 @@ int launch_gemm(const GemmArgs &a, int grid, size_t smem, const Maps &maps, int 
   cfg.attrs = at;
   cfg.numAttrs = a.cs > 1 ? 2 : 1;
   prof_begin(FFN_B200_K_INT8_GEMM, st);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_kernel<T, PAIR>, a, maps);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_kernel<T>, a, maps);
   prof_end(FFN_B200_K_INT8_GEMM, st);
   note_launch();
   if (e != cudaSuccess) {
@@ -753,7 +695,6 @@ struct GemmPlan {
   Maps maps;
   size_t smem;
   int grid, dev;
-  bool pair;  // CTA pairs on tiles of 256 channels
 };
 int plan_gemm(GemmPlan &p, size_t rows, size_t n, size_t k, size_t n_groups, const int32_t *offsets, const int8_t *x,
               size_t ld_x, const float *x_scales, const int8_t *w, size_t ld_w, const float *w_scales, const float *bias,
@@ -783,87 +724,66 @@ int plan_gemm(GemmPlan &p, size_t rows, size_t n, size_t k, size_t n_groups, con
   a.rows = (int)rows, a.n = (int)n, a.groups = (int)n_groups;
   a.kt = (int)((k + kKB - 1) / kKB);
   a.kfull = (int)(k / kKB);
-  const long long ct1 = (long long)((n + kM - 1) / kM), ct2 = (long long)((n + 2 * kM - 1) / (2 * kM));
+  const long long ct = (long long)((n + kM - 1) / kM);
   a.cs = 1;
   if (offsets) {
     // Groups: bound by the weights' bytes, so one chunk should hold a group: the
-    // average and three deviations of an even routing (48 experts, 128 rows each:
-    // 89.5 us with 192 rows a tile, 92.9 with 160, 90.6 with 256; 8 rows each: 122
-    // us with 32 rows, 125 with 16).
+    // average and three deviations of an even routing (48 experts of 8 rows each:
+    // 122 us with 32 rows a tile, 125 with 16).
     const double avg = (double)rows / n_groups, want = avg + 3 * sqrt(avg);
     a.nt = want <= 16 ? 16 : want >= 256 ? 256 : ((int)ceil(want) + 31) / 32 * 32;
-    p.pair = a.nt > 128 && n > (size_t)kM;
-    if (!p.pair) a.nt = std::min(a.nt, 128);
   } else {
-    // One matrix: the cheapest of the tiles by waves x blocks of K x time a block,
-    // in us as measured at 4096 x 4096 (single CTA 0.10 + 0.0029 a token, pair 0.12
-    // + 0.00135; 77 rows x 5120 x 2304: 9.5 us with 16 rows a tile, 11.5 with 32,
-    // 12.9 with 48; 512 x 4096 x 4096: pairs of 128 rows 14.1, single 128 rows
-    // 18.8).  K split over a cluster costs 3.5 us more than it saves in blocks, and
-    // pays for few channels and a long K (16 x 8192 x 1024: 7.9 us, 11.9 without).
+    // One matrix: the cheapest tile by waves x blocks of K x time a block (0.10 +
+    // 0.0029 us a token, measured at 4096 x 4096; 77 rows x 5120 x 2304: 9.5 us with
+    // 16 rows a tile, 11.5 with 32, 12.9 with 48).  K split over a cluster costs
+    // 3.5 us more than it saves in blocks, and pays for few channels and a long K
+    // (16 x 8192 x 1024: 7.9 us, 11.9 without).
     double best = 1e300;
-    auto consider = [&](int nt, bool pair, int cs) {
-      const int chunks = (int)((rows + nt - 1) / nt), round = pair ? 32 : 16;
-      const double per = (double)((rows + chunks - 1) / chunks + round - 1) / round * round;
-      const double tiles = (double)chunks * (pair ? ct2 : ct1);
-      const double waves = cs > 1 ? 1 : ceil(tiles / (pair ? sms / 2 : sms));
-      double us = waves * ceil((double)a.kt / cs) * (pair ? 0.12 + 0.00135 * per : 0.10 + 0.0029 * per);
-      if (cs > 1) us += 3.5 + 0.02 * per;
-      if (us < best) best = us, a.nt = nt, p.pair = pair, a.cs = cs;
-    };
-    for (int nt : {16, 32, 48, 64, 96, 128}) {
-      consider(nt, false, 1);
-      // clusters that are sure to be resident at once
-      const long long tiles = ct1 * (long long)((rows + nt - 1) / nt);
-      for (int cs = 2; cs <= 8 && tiles * cs <= sms * 3 / 4 && a.kt >= 4 * cs; cs *= 2) consider(nt, false, cs);
+    for (int nt : {16, 32, 48, 64, 96, 128, 192, 256}) {
+      const long long chunks = (long long)((rows + nt - 1) / nt), tiles = ct * chunks;
+      const long long per = ((long long)rows + chunks - 1) / chunks, n16 = (per + 15) / 16 * 16;
+      const double block = 0.10 + 0.0029 * (double)n16;
+      for (int cs = 1; cs <= 8; cs *= 2) {
+        // (clusters that are sure to be resident at once)
+        if (cs > 1 && (nt > kSplitRows || tiles * cs > sms * 3 / 4 || a.kt < 4 * cs)) break;
+        const double us = cs == 1 ? ceil((double)tiles / sms) * a.kt * block
+                                  : ceil((double)a.kt / cs) * block + 3.5 + 0.02 * (double)n16;
+        if (us < best) best = us, a.nt = nt, a.cs = cs;
+      }
       if ((size_t)nt >= rows) break;
     }
-    if (n > (size_t)kM && rows > 64)
-      for (int nt : {128, 160, 192, 224, 256}) consider(nt, true, 1);
   }
-  if (p.pair) a.cs = 2;
-  const long long ct = p.pair ? ct2 : ct1;
   // tiles at most: each group may end in a partial chunk
   const long long chunks = offsets ? std::min<long long>(rows, rows / a.nt + n_groups) : (rows + a.nt - 1) / a.nt;
   const long long tiles = ct * chunks;
   // (the kernel's tile numbers stay in 32 bits even where offsets are not ascending)
   if ((double)(rows / a.nt + 1) * (double)n_groups * (double)ct > 2147483647.0) return fail(FFN_B200_EINVAL, "int8_matmul: too many tiles");
-  const size_t tail = (!p.pair && a.cs > 1 ? (size_t)kM * a.nt * 4 : 0) + (3 * n_groups + 1) * sizeof(int);
-  const size_t block = (size_t)kABytes + (size_t)(p.pair ? a.nt / 2 : a.nt) * kKB, room = kSmemMax - 1024 - tail;
-  // as many blocks a stage, up to 4, as leave three stages (four for pairs): each
-  // costs its threads a wait and a commit (64 blocks, 16 rows: 12.1 us with 4 a
-  // stage, 18.9 with 1), and DRAM likes the rows' bytes together
+  const size_t tail = (a.cs > 1 ? (size_t)kM * a.nt * 4 : 0) + (3 * n_groups + 1) * sizeof(int);
+  const size_t block = (size_t)kABytes + (size_t)a.nt * kKB, room = kSmemMax - 1024 - tail;
+  // as many blocks a stage, up to 4, as leave three stages: each costs its threads
+  // a wait and a commit (64 blocks, 16 rows: 12.1 us with 4 a stage, 18.9 with 1),
+  // and DRAM likes the rows' bytes together
   a.sub = 4;
-  while (a.sub > 1 && ((p.pair ? 4 : 3) * a.sub * block > room || a.kt < 2 * a.sub * (p.pair ? 1 : a.cs))) --a.sub;
+  while (a.sub > 1 && (3 * a.sub * block > room || a.kt < 2 * a.sub * a.cs)) --a.sub;
   const size_t stage = a.sub * block;
   a.stages = (int)std::min<size_t>({room / stage, (size_t)kMaxStages, (size_t)std::max(2, a.kt)});
   if (a.stages < 2) return fail(FFN_B200_EUNSUP, "int8_matmul: too many groups for shared memory");
   p.smem = 1024 + a.stages * stage + tail;
-  // A pair waits for the TMEM of both its SMs at once.  It takes so much shared
-  // memory that no CTA of a K-splitting cluster fits beside it, so the two never
-  // wait for each other's columns.
-  if (p.pair) p.smem = std::max<size_t>(p.smem, 196 * 1024);
-  const int xr = p.pair ? a.nt / 2 : a.nt;
   if (a.kfull) {
     if (int rc = encode(&p.maps.w3, w, n_groups * n, k, ld_w, kM, a.sub)) return rc;
-    if (int rc = encode(&p.maps.x3, x, rows, k, ld_x, xr, a.sub)) return rc;
+    if (int rc = encode(&p.maps.x3, x, rows, k, ld_x, a.nt, a.sub)) return rc;
   }
   if (a.kfull < a.kt) {
     if (int rc = encode(&p.maps.w2, w, n_groups * n, k, ld_w, kM, 0)) return rc;
-    if (int rc = encode(&p.maps.x2, x, rows, k, ld_x, xr, 0)) return rc;
+    if (int rc = encode(&p.maps.x2, x, rows, k, ld_x, a.nt, 0)) return rc;
   }
-  p.grid = p.pair ? 2 * (int)std::min<long long>(tiles, sms / 2) : a.cs > 1 ? (int)tiles * a.cs : (int)std::min<long long>(tiles, sms);
+  p.grid = a.cs > 1 ? (int)tiles * a.cs : (int)std::min<long long>(tiles, sms);
   return 0;
 }
-template <typename T>
-int run_gemm_as(const GemmPlan &p, cudaStream_t st) {
-  return p.pair ? launch_gemm<T, true>(p.a, p.grid, p.smem, p.maps, p.dev, st)
-                : launch_gemm<T, false>(p.a, p.grid, p.smem, p.maps, p.dev, st);
-}
 int run_gemm(const GemmPlan &p, int32_t dtype, cudaStream_t st) {
-  if (dtype == FFN_B200_DT_F32) return run_gemm_as<float>(p, st);
-  if (dtype == FFN_B200_DT_BF16) return run_gemm_as<__nv_bfloat16>(p, st);
-  return run_gemm_as<__half>(p, st);
+  if (dtype == FFN_B200_DT_F32) return launch_gemm<float>(p.a, p.grid, p.smem, p.maps, p.dev, st);
+  if (dtype == FFN_B200_DT_BF16) return launch_gemm<__nv_bfloat16>(p.a, p.grid, p.smem, p.maps, p.dev, st);
+  return launch_gemm<__half>(p.a, p.grid, p.smem, p.maps, p.dev, st);
 }
 
 template <typename T, int VEC, bool SWIGLU>
