@@ -484,13 +484,13 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
 }
 
 // ------------------------------------------- few tokens, quantised in place
-// A decode step of 1 to 4 tokens against one matrix: a single launch.  Every CTA
+// A decode step of one or two tokens against one matrix: a single launch.  Every CTA
 // quantises the tokens for itself (a few KB, L2 hits) while its warps' first
 // weights are on the way; a warp then takes a channel at a time, 16 bytes a
 // lane and load, and multiplies with dp4a.  Bound by the weights' bytes: 128 KB
 // of loads in flight an SM.
-constexpr int kFewRows = 4;
-constexpr int kFewThreads = 256;
+constexpr int kFewRows = 2;
+constexpr int kFewThreads = 512;
 constexpr size_t kFewSmem = 47 * 1024;  // the launch default, less the static part
 struct FewArgs {
   const void *x;
@@ -536,9 +536,9 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(const FewArgs a) {
       if (ch < a.n && 16 * p < a.k) w[j] = few_piece(a.w + (size_t)ch * a.ld_w, p, a.k);
     }
   };
-  load(c, 0);
 
-  // quantise: largest magnitudes, then codes
+  // quantise: largest magnitudes, then codes.  The tokens are read before the
+  // weights are asked for: behind 100 KB of weights an SM they came last.
   uint32_t m[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
@@ -551,6 +551,7 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(const FewArgs a) {
     m[r] = __reduce_max_sync(0xffffffffu, m[r]);
     if (lane == 0) s_max[r][warp] = m[r];
   }
+  load(c, 0);
   __syncthreads();
   float scale[R];
 #pragma unroll
@@ -618,9 +619,7 @@ int launch_few(const FewArgs &a, int rows, int sms, cudaStream_t st) {
   const size_t smem = (size_t)rows * few_pitch(a.k);
 #define FFN_GO(R) FFN_LAUNCH_PDL(FFN_B200_K_INT8_GEMM, st, "int8_linear", (few_kernel<T, R>), grid, kFewThreads, smem, a)
   if (rows == 1) FFN_GO(1);
-  else if (rows == 2) FFN_GO(2);
-  else if (rows == 3) FFN_GO(3);
-  else FFN_GO(4);
+  else FFN_GO(2);
 #undef FFN_GO
   return 0;
 }

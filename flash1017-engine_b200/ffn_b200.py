@@ -820,17 +820,33 @@ class MoeLayer:
 #
 # One call is one or two kernel launches of a few microseconds, so the checks
 # stay lean: torch's accessors below cost 0.1 us each, current_stream() 2.
+# The plain cases go through a CPython module (csrc/torch_calls.cpp) that makes
+# the outputs and calls the library; what it does not take (None) and everything
+# where it was not built comes through here.
+CALLS_PATH = os.path.join(HERE, "_build", "ffn_b200_torch.so")
 _dts = None
-_T = _dev_now = _raw_stream = None
+_T = _dev_now = _raw_stream = _calls = None
 
 
 def _setup():
-    global _T, _dts, _dev_now, _raw_stream
+    global _T, _dts, _dev_now, _raw_stream, _calls
     import torch
     _dts = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
     _dev_now, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
     lib()
+    if os.path.exists(CALLS_PATH):
+        import importlib.util
+        spec = importlib.util.spec_from_file_location("ffn_b200_torch", CALLS_PATH)
+        _calls = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(_calls)
     _T = torch
+
+
+def _answer(r, what):
+    """An entry point's answer through the module: tensors, or its error."""
+    if type(r) is int:
+        check(r, what)
+    return r
 
 
 def _dtype(dtype):
@@ -983,6 +999,11 @@ class Int8Matrix:
         type, x's, or float32 for codes.  Several groups: offsets int32 [groups
         + 1], tokens offsets[g] .. offsets[g + 1] - 1 take group g, the others'
         rows are left as they were."""
+        if _calls is not None and out is None and dtype is None and stream is None and type(x) is not tuple:
+            r = _calls.int8_linear(self.w, self.ld, self.scale, self.bias, self.groups, self.rows, self.cols, x,
+                                   offsets)
+            if r is not None:
+                return _answer(r, "int8_matmul")
         floats = not isinstance(x, (tuple, list))
         first = x if floats else x[0]
         dev = _dev(first, stream)
@@ -1037,6 +1058,10 @@ def moe_sort(idx, expert_begin, expert_end, stream=None):
     the experts [expert_begin, expert_end) only: (offsets [experts + 1], pos
     [tokens, top_k] with -1 elsewhere, src [tokens * top_k] with -1 behind the
     last row), all int32 (ffn_b200_moe_sort)."""
+    if _calls is not None and stream is None:
+        r = _calls.moe_sort(idx, expert_begin, expert_end)
+        if r is not None:
+            return _answer(r, "moe_sort")
     dev = _dev(idx, stream)
     if dev < 0:
         with _on(idx, stream):
@@ -1062,6 +1087,10 @@ def moe_permute(x, pos, out=None, scales=None, out_scales=None, stream=None):
     """out[pos[t, k]] = x[t] for rows of any type (ffn_b200_moe_permute); new
     rows: one per pair.  With scales f32 [tokens] (int8 rows): (out,
     out_scales).  Rows that no pair names are left as they were."""
+    if _calls is not None and stream is None and scales is None and out_scales is None:
+        r = _calls.moe_permute(x, pos, out)
+        if r is not None:
+            return _answer(r, "moe_permute")
     dev = _dev(x, stream)
     if dev < 0:
         with _on(x, stream):
@@ -1097,6 +1126,10 @@ def moe_permute(x, pos, out=None, scales=None, out_scales=None, stream=None):
 def moe_combine(y, pos, weight=None, residual=None, out=None, stream=None):
     """out[t] = residual[t] + sum_k weight[t, k] y[pos[t, k]] (weight f32
     [tokens, top_k] or None: 1), in f32, rounded once (ffn_b200_moe_combine)."""
+    if _calls is not None and stream is None and out is None:
+        r = _calls.moe_combine(y, pos, weight, residual)
+        if r is not None:
+            return _answer(r, "moe_combine")
     dev = _dev(y, stream)
     if dev < 0:
         with _on(y, stream):
@@ -1182,6 +1215,10 @@ class BlockNorm:
         """(h, xn), each a new tensor or the one given; y None: the residual
         alone.  codes True: (h, xn, codes, scales) with xn None unless given and
         the int8 codes of xn (quantize_int8 of its f32 values)."""
+        if _calls is not None and y is not None and h is None and xn is None and not codes and stream is None:
+            r = _calls.block_norm(self.pre_w, self.post_w, self.alpha, self.beta, self.eps, y, residual, gate)
+            if r is not None:
+                return _answer(r, "block_norm")
         like = residual if y is None else y
         if like is None:
             raise FfnError("BlockNorm: neither y nor residual")

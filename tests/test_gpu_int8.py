@@ -325,3 +325,40 @@ def test_streams_graphs_and_a_block_from_norm_to_norm(ffn, cuda):
     torch.cuda.synchronize()
     for _, out in graphs:
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_calls_with_and_without_the_module(ffn, cuda, monkeypatch):
+    """The CPython module and the ctypes path: the same bits, and refusals of
+    the same calls."""
+    import torch
+    T, H, E, K = 21, 200, 12, 3
+    g = torch.Generator(device=cuda).manual_seed(1)
+    x = torch.randn(T, H, device=cuda, generator=g).to(torch.float16)
+    w = ffn.Int8Matrix(torch.randint(-127, 128, (E, 40, H), device=cuda, generator=g, dtype=torch.int8),
+                       torch.rand(E, 40, device=cuda, generator=g) * 0.01, torch.randn(E, 40, device=cuda, generator=g))
+    idx = torch.randint(0, E + 3, (T, K), device=cuda, generator=g, dtype=torch.int32)
+    wt, gate = torch.rand(T, K, device=cuda, generator=g), torch.rand(T, 1, device=cuda, generator=g)
+    p = torch.rand(H, device=cuda, generator=g)
+    ffn.quantize_int8(x)
+    assert ffn._calls is not None
+
+    def run():
+        off, pos, src = ffn.moe_sort(idx, 2, E + 2)
+        xs = ffn.moe_permute(x, pos, out=torch.zeros(T * K, H, dtype=x.dtype, device=cuda))
+        y = ffn.Int8Matrix(w.w, w.scale, w.bias).matmul(xs, offsets=off)[:int(off[-1])]
+        back = ffn.moe_combine(xs, pos, wt, residual=x)
+        return [off, pos, src, xs, y, back, *ffn.BlockNorm(p, p, 0.5, 2.0).forward(back, x, gate=gate),
+                *ffn.BlockNorm(None, p).forward(x)[:1], *ffn.BlockNorm(p).forward(x, gate=p)]
+    refused = [lambda: ffn.moe_sort(idx, 5, 5), lambda: ffn.moe_sort(idx, -1, 5), lambda: ffn.moe_combine(x, idx.long()),
+               lambda: ffn.moe_permute(x[:3], idx), lambda: w.matmul(x), lambda: w.matmul(x[:, :100]),
+               lambda: ffn.BlockNorm(p[:9]).forward(x, x), lambda: ffn.BlockNorm(p).forward(x, x.float()),
+               lambda: ffn.BlockNorm(p, eps=-1.0).forward(x, x), lambda: ffn.moe_combine(x, idx, wt.half())]
+    fast = run()
+    for call in refused:
+        with pytest.raises(ffn.FfnError):
+            call()
+    monkeypatch.setattr(ffn, "_calls", None)
+    assert all(torch.equal(a, b) for a, b in zip(fast, run()))
+    for call in refused:
+        with pytest.raises(ffn.FfnError):
+            call()

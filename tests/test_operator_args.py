@@ -152,3 +152,21 @@ def test_python_wrappers_refuse_before_the_library(ffn):
                  lambda: ffn.Int8Matrix(x, torch.ones(4))):
         with pytest.raises(ffn.FfnError):
             call()
+
+
+def test_the_module_of_calls_is_built_and_leaves_what_it_does_not_take(ffn):
+    """CPU tensors, wrong types and wrong counts: None, so that the Python path
+    refuses them; the module holds the five calls of small kernels."""
+    import torch
+    ffn._setup()
+    m = ffn._calls
+    assert m is not None
+    x, i32 = torch.zeros(4, 64), torch.zeros(4, 2, dtype=torch.int32)
+    assert m.block_norm(None, None, 1.0, 1.0, 0.0, x, None, None) is None
+    assert m.block_norm(None, None, 1.0, 1.0, 0.0, None, None, None) is None
+    assert m.block_norm(None, None, "a", 1.0, 0.0, 3, None, None) is None
+    assert m.int8_linear(x, 64, x, None, 1, 4, 64, x, None) is None
+    assert m.moe_sort(i32, 0, 8) is None and m.moe_permute(x, i32, None) is None
+    assert m.moe_combine(x, i32, None, None) is None
+    with pytest.raises(TypeError):
+        m.moe_sort(i32, 0)
