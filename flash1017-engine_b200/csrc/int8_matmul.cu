@@ -46,61 +46,88 @@ __device__ __forceinline__ float swiglu10(float g, float u) {
   return fminf(__fdividef(g, 1.0f + expf(-g)), 10.0f) * fminf(fmaxf(u, -10.0f), 10.0f);
 }
 
-template <typename T, int VEC, int NV, bool WARP, bool SWIGLU>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) quant_kernel(const QuantArgs a) {
-  __shared__ uint32_t s_red[32];
+// Persistent, a row per CTA at a time; thread l holds the columns of pieces l, l +
+// L, ... (16 in all) and has its pieces of the CTA's next two rows brought into
+// shared memory meanwhile (STAGED).  A CTA a row took 22 us for 8192 x 4096 bf16
+// (4.5 TB/s), 21 us like this.
+constexpr int kQuantStages = 3;
+template <typename T, int VEC, int NV, int MT, bool SWIGLU, bool STAGED>
+__global__ void __launch_bounds__(MT) quant_kernel(const QuantArgs a) {
+  constexpr int W = SWIGLU ? 2 : 1;  // gate and up
+  __shared__ uint32_t s_red[2][32];
+  extern __shared__ __align__(16) uint8_t s_dyn[];  // stages [kQuantStages][W][NV][threads] of 16 bytes
   pdl_enter();
-  const uint32_t l = WARP ? threadIdx.x & 31 : threadIdx.x, L = WARP ? 32 : blockDim.x;
-  const long long row = WARP ? (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
-  if (row >= a.rows || (a.n_rows && row >= __ldg(a.n_rows))) return;
-  const T *xr = (const T *)a.x + (size_t)row * a.ld_x;
-  Raw<T, VEC> rx[NV], ru[NV];
+  const uint32_t l = threadIdx.x, L = blockDim.x;
+  const int lane = l & 31, warp = l >> 5, nw = L >> 5;
+  const int rows = a.n_rows ? min(a.rows, __ldg(a.n_rows)) : a.rows;
+  uint4 *st = reinterpret_cast<uint4 *>(s_dyn) + l;
+  auto fetch = [&](int stage, long long row) {
+    if (row < rows) {
+      const T *p = (const T *)a.x + (size_t)row * a.ld_x;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const uint32_t v = l + i * L;
-    if (v < a.n_vec) {
-      rx[i] = load_raw<T, VEC>(xr, v);
-      if (SWIGLU) ru[i] = load_raw<T, VEC>(xr + a.cols, v);
+      for (int w = 0; w < W; ++w)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (l + i * L < a.n_vec)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tc::sa(st + ((stage * W + w) * NV + i) * L)),
+                         "l"(p + (size_t)w * a.cols + (l + i * L) * VEC) : "memory");
     }
-  }
-  float f[SWIGLU ? NV : 1][VEC];
-  uint32_t m = 0;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (STAGED)
+    for (int q = 0; q < kQuantStages - 1; ++q) fetch(q, blockIdx.x + (long long)q * gridDim.x);
+  int par = 0, stage = 0;
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x, par ^= 1) {
+    Raw<T, VEC> r[W][NV];
+    if constexpr (STAGED) {
+      fetch(stage == 0 ? kQuantStages - 1 : stage - 1, row + (long long)(kQuantStages - 1) * gridDim.x);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kQuantStages - 1) : "memory");
+    }
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const uint32_t v = l + i * L;
-    if (v >= a.n_vec) continue;
-    if (SWIGLU) {
-      float u[VEC];
-      unpack<T, VEC>(rx[i], f[i]);
-      unpack<T, VEC>(ru[i], u);
+    for (int w = 0; w < W; ++w)
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        // the clamps would hide a gate or an up that is not finite
-        const bool fin = isfinite(f[i][j]) && isfinite(u[j]);
-        f[i][j] = swiglu10(f[i][j], u[j]);
-        m = max(m, fin ? __float_as_uint(f[i][j]) & 0x7fffffffu : 0x7f800000u);
+      for (int i = 0; i < NV; ++i)
+        if (l + i * L < a.n_vec) {
+          if constexpr (STAGED) r[w][i] = *reinterpret_cast<const Raw<T, VEC> *>(st + ((stage * W + w) * NV + i) * L);
+          else r[w][i] = load_raw<T, VEC>((const T *)a.x + (size_t)row * a.ld_x + (size_t)w * a.cols, l + i * L);
+        }
+    stage = stage == kQuantStages - 1 ? 0 : stage + 1;
+    float f[SWIGLU ? NV : 1][VEC];
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (l + i * L >= a.n_vec) continue;
+      if (SWIGLU) {
+        float u[VEC];
+        unpack<T, VEC>(r[0][i], f[i]);
+        unpack<T, VEC>(r[W - 1][i], u);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          // the clamps would hide a gate or an up that is not finite
+          const bool fin = isfinite(f[i][j]) && isfinite(u[j]);
+          f[i][j] = swiglu10(f[i][j], u[j]);
+          m = max(m, fin ? __float_as_uint(f[i][j]) & 0x7fffffffu : 0x7f800000u);
+        }
+      } else {
+        m = max(m, abs_bits<T, VEC>(r[0][i]));
       }
-    } else {
-      m = max(m, abs_bits<T, VEC>(rx[i]));
     }
-  }
-  m = __reduce_max_sync(0xffffffffu, m);
-  if (!WARP) {
-    const int lane = threadIdx.x & 31, nw = blockDim.x >> 5;
-    if (lane == 0) s_red[threadIdx.x >> 5] = m;
-    __syncthreads();
-    m = __reduce_max_sync(0xffffffffu, lane < nw ? s_red[lane] : 0u);
-  }
-  const Int8Row sc(SWIGLU ? __uint_as_float(m) : from_abs_bits<T>(m));
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (nw > 1) {
+      if (lane == 0) s_red[par][warp] = m;
+      __syncthreads();
+      m = __reduce_max_sync(0xffffffffu, lane < nw ? s_red[par][lane] : 0u);
+    }
+    const Int8Row sc(SWIGLU ? __uint_as_float(m) : from_abs_bits<T>(m));
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const uint32_t v = l + i * L;
-    if (v >= a.n_vec) continue;
-    float e[VEC];
-    if (!SWIGLU) unpack<T, VEC>(rx[i], e);
-    store_codes<VEC>(a.codes + (size_t)row * a.ld_c + (size_t)v * VEC, SWIGLU ? f[SWIGLU ? i : 0] : e, sc);
+    for (int i = 0; i < NV; ++i) {
+      if (l + i * L >= a.n_vec) continue;
+      float e[VEC];
+      if (!SWIGLU) unpack<T, VEC>(r[0][i], e);
+      store_codes<VEC>(a.codes + (size_t)row * a.ld_c + (size_t)(l + i * L) * VEC, SWIGLU ? f[SWIGLU ? i : 0] : e, sc);
+    }
+    if (l == 0) a.scales[row] = sc.scale();
   }
-  if (l == 0) a.scales[row] = sc.scale();
 }
 
 // ----------------------------------------------------------------- product
@@ -109,8 +136,8 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) quant_kernel(const QuantArg
 // dividing: two divisions a stage cost more than its waits and copies together
 // (8192 x 4096 x 4096: 97 us with them, 94 us without).
 constexpr int kMmaWarp = 1;
-constexpr int kThreads = 192;
-constexpr int kM = 128;             // channels a tile
+__host__ __device__ constexpr int threads_of(int mb) { return 64 + 128 * mb; }  // four epilogue warps a block of channels
+constexpr int kM = 128;             // channels a block; a tile has one or two (MB)
 constexpr int kKB = 128;            // K bytes (= values) a stage
 constexpr int kABytes = kM * kKB;
 constexpr int kMaxStages = 12;
@@ -216,13 +243,14 @@ __device__ __forceinline__ void st_peer(const void *p, uint32_t rank, int v) {
   asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(b), "r"(v) : "memory");
 }
 
-// One tile: 128 channels of group g from channel c0, tokens [r0, r0 + nn).
+// One tile: 128 MB channels of group g from channel c0, tokens [r0, r0 + nn).
 struct Tile {
   int g, c0, r0, nn;
 };
 // s_pre[g]: token chunks of the groups before g.  Tiles run over the groups,
 // inside a group over the channel blocks, inside a block over its token chunks,
 // so CTAs that run together share the weights' block.
+template <int MB>
 __device__ __forceinline__ Tile tile_of(int t, const GemmArgs &a, const int *s_pre, const int *s_off, int ct) {
   int lo = 0, hi = a.groups;  // the last g with s_pre[g] * ct <= t
   while (hi - lo > 1) {
@@ -236,25 +264,30 @@ __device__ __forceinline__ Tile tile_of(int t, const GemmArgs &a, const int *s_p
   const int j = rel % chunks;
   Tile o;
   o.g = lo;
-  o.c0 = rel / chunks * kM;
+  o.c0 = rel / chunks * (MB * kM);
   o.r0 = first + j * per;
   o.nn = max(0, min(per, n - j * per));
   return o;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, const __grid_constant__ Maps maps) {
+// MB = 2 halves the tokens' share of the traffic: with 128 x 256 tiles a dense
+// prefill moves 48 KB a block of K from L2, 14 TB/s, which is what L2 gives; 256 x
+// 256 tiles move 64 KB for twice the products.  Their two accumulators fill TMEM,
+// so a tile's epilogue (eight warps) is not hidden behind the next one's MMAs.
+template <typename T, int MB>
+__global__ void __launch_bounds__(threads_of(MB), 1) gemm_kernel(const GemmArgs a, const __grid_constant__ Maps maps) {
+  constexpr int kThreads = threads_of(MB), kBufs = MB == 1 ? 2 : 1, kWBytes = MB * kABytes;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], mma_done;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_err, s_sum[kThreads / 32];
+  __shared__ int s_err, s_sum[threads_of(MB) / 32];
   __shared__ float s_xs[kSplitRows];
   uint8_t *smem = smem_raw + ((1024 - (tc::sa(smem_raw) & 1023)) & 1023);
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   // a stage: sub blocks of weights, then sub blocks of tokens
-  const int x_bytes = a.nt * kKB, stage_bytes = a.sub * (kABytes + x_bytes);
+  const int x_bytes = a.nt * kKB, stage_bytes = a.sub * (kWBytes + x_bytes);
   int *red = reinterpret_cast<int *>(smem + a.stages * stage_bytes);     // cs > 1: [cs][nt][128 / cs]
-  const bool split = a.cs > 1;
+  const bool split = MB == 1 && a.cs > 1;
   int *s_off = red + (split ? kM * a.nt : 0);                          // [groups][first, count]
   int *s_pre = s_off + 2 * a.groups;                                      // [groups + 1]
   // two accumulators; one where a cluster has a single tile.  At most 64 columns
@@ -262,12 +295,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
   // waited for each other's TMEM on two SMs would wait for good.
   const int acc_cols = a.nt <= 16 ? 16 : 1 << (32 - __clz(a.nt - 1)), tmem_cols = split ? max(32, acc_cols) : 2 * acc_cols;
   const uint32_t rank = a.cs > 1 ? ctarank() : 0;
-  const int ct = (a.n + kM - 1) / kM;
+  const int ct = (a.n + MB * kM - 1) / (MB * kM);
 
   if (tid == 0) {
     s_err = 0;
     for (int s = 0; s < a.stages; ++s) { tc::bar_init(&full[s], 1); tc::bar_init(&empty[s], 1); }
-    for (int b = 0; b < 2; ++b) { tc::bar_init(&acc_full[b], 1); tc::bar_init(&acc_empty[b], 4); }
+    for (int b = 0; b < 2; ++b) { tc::bar_init(&acc_full[b], 1); tc::bar_init(&acc_empty[b], 4 * MB); }
     tc::bar_init(&mma_done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (a.kfull) {
@@ -283,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
     // has finished; bring them into L2 (a hint, nothing is read from it yet)
     const int chunks = (a.rows + a.nt - 1) / a.nt;
     if (tile0 < chunks * ct)
-      tma_prefetch_l2(&maps.w3, tile0 / chunks * kM, k_lo + lane * a.sub);
+      tma_prefetch_l2(&maps.w3, tile0 / chunks * MB * kM, k_lo + lane * a.sub);
   }
   pdl_enter();
 
@@ -330,24 +363,24 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
       uint32_t ph = 0, used = 0;  // the stage, its phase, the stages ever used
       bool live = true;
       for (int t = tile0; t < n_tiles && live; t += tile_step) {
-        const Tile o = tile_of(t, a, s_pre, s_off, ct);
+        const Tile o = tile_of<MB>(t, a, s_pre, s_off, ct);
         const int ch = o.g * a.n + o.c0;
         for (int k = k_lo; k < k_hi; k += a.sub) {
           if (!wait_bar(&empty[s], ph ^ 1, &s_err, 1)) { live = false; break; }
-          uint8_t *sw = smem + s * stage_bytes, *sx = sw + a.sub * kABytes;
+          uint8_t *sw = smem + s * stage_bytes, *sx = sw + a.sub * kWBytes;
           // One copy for all blocks of a stage: a single thread issues them, and
           // with a copy per block and per 32 tokens it was what the kernel waited
           // for (8192 x 4096 x 4096: 145 us; one box of 128 tokens 124 us).  Blocks
           // past the last full one read as zeros.
           const bool tail = a.kfull < a.kt && k + a.sub > a.kfull;
           const int n = tail ? min(a.sub, k_hi - k) : a.sub;
-          tc::bar_arrive_tx(&full[s], n * (kABytes + x_bytes));
+          tc::bar_arrive_tx(&full[s], n * (kWBytes + x_bytes));
           if (!tail) {
             tma_3d(sw, &maps.w3, ch, k, &full[s]);
             tma_3d(sx, &maps.x3, o.r0, k, &full[s]);
           } else {
             for (int q = 0; q < n; ++q) {
-              tma_2d(sw + q * kABytes, &maps.w2, (k + q) * kKB, ch, &full[s]);
+              tma_2d(sw + q * kWBytes, &maps.w2, (k + q) * kKB, ch, &full[s]);
               tma_2d(sx + q * x_bytes, &maps.x2, (k + q) * kKB, o.r0, &full[s]);
             }
           }
@@ -368,16 +401,16 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
       // low field and stays below its 14 bits.  elect.sync rather than a lane
       // number lets the compiler keep all of this in uniform registers, which is
       // where the instruction wants it.
-      const uint64_t w0 = tc::desc_sw128(tc::sa(smem)), x0 = tc::desc_sw128(tc::sa(smem) + a.sub * kABytes);
+      const uint64_t w0 = tc::desc_sw128(tc::sa(smem)), x0 = tc::desc_sw128(tc::sa(smem) + a.sub * kWBytes);
       uint64_t dw = w0, dx = x0;
       int s = 0, n = 0;
       uint32_t ph = 0;
       bool live = true;
       for (int t = tile0; t < n_tiles && live; t += tile_step, ++n) {
-        const Tile o = tile_of(t, a, s_pre, s_off, ct);
+        const Tile o = tile_of<MB>(t, a, s_pre, s_off, ct);
         const uint32_t id = idesc_i8(kM, (o.nn + 15) & ~15);
-        const int b = n & 1;
-        if (!wait_bar(&acc_empty[b], ((n >> 1) & 1) ^ 1, &s_err, 2)) break;
+        const int b = n % kBufs;
+        if (!wait_bar(&acc_empty[b], ((n / kBufs) & 1) ^ 1, &s_err, 2)) break;
         tc::fence_after();
         const uint32_t d = tmem + b * acc_cols;
         uint32_t acc = 0;
@@ -386,9 +419,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
           if (!wait_bar(&full[s], ph, &s_err, 3)) { live = false; break; }
           tc::fence_after();
           uint64_t qw = dw, qx = dx;
-          for (int q = 0; q < nq; ++q, qw += kABytes >> 4, qx += x_bytes >> 4) {
+          for (int q = 0; q < nq; ++q, qw += kWBytes >> 4, qx += x_bytes >> 4) {
 #pragma unroll
-            for (int j = 0; j < kKB / 32; ++j, acc = 1) mma_i8(d, qw + 2 * j, qx + 2 * j, id, acc);
+            for (int j = 0; j < kKB / 32; ++j, acc = 1)
+#pragma unroll
+              for (int mi = 0; mi < MB; ++mi)
+                mma_i8(d + mi * acc_cols, qw + mi * (kABytes >> 4) + 2 * j, qx + 2 * j, id, acc);
           }
           tc::commit(&empty[s]);
           dw += stage_bytes >> 4, dx += stage_bytes >> 4;
@@ -403,15 +439,29 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
     __syncwarp();
   } else {
     // -------------------------------------------------- epilogue (4 warps)
-    const int quarter = warp & 3, cl = quarter * 32 + lane;
+    // the second four of MB = 2 take the second block of channels
+    const int quarter = warp & 3, mi = (warp - kMmaWarp - 1) >> 2, cl = quarter * 32 + lane;
     int n = 0;
     if (split) cluster_wait();
     for (int t = tile0; t < n_tiles; t += tile_step, ++n) {
-      const Tile o = tile_of(t, a, s_pre, s_off, ct);
-      const int b = n & 1;
-      const bool ok = __any_sync(0xffffffffu, lane == 0 && wait_bar(&acc_full[b], (n >> 1) & 1, &s_err, 4));
+      const Tile o = tile_of<MB>(t, a, s_pre, s_off, ct);
+      const int b = n % kBufs, ch = o.c0 + mi * kM + cl;
+      const bool on = ch < a.n;
+      // the scales, before the wait: column 32 i + lane's in xs[i].  Asked for in
+      // the loop, their latency was a third of a tile with a short K (6144 x 1024 x
+      // 4096 over 48 groups: 114 us, 48 us like this).
+      float xs[8], sw = 0.f, bias = 0.f;
+      if (!split) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) xs[i] = 32 * i + lane < o.nn ? __ldg(a.xs + o.r0 + 32 * i + lane) : 0.f;
+        if (on) {
+          sw = __ldg(a.ws + (size_t)o.g * a.n + ch);
+          if (a.bias) bias = __ldg(a.bias + (size_t)o.g * a.n + ch);
+        }
+      }
+      const bool ok = __any_sync(0xffffffffu, lane == 0 && wait_bar(&acc_full[b], (n / kBufs) & 1, &s_err, 4));
       tc::fence_after();
-      const uint32_t tl = tmem + b * acc_cols + ((uint32_t)(32 * quarter) << 16);
+      const uint32_t tl = tmem + (MB == 1 ? b : mi) * acc_cols + ((uint32_t)(32 * quarter) << 16);
       if (split) {
         // this CTA's part of K: lane cl's sums go to the CTA that owns the channel
         const int own = kM / a.cs, dst = cl / own;
@@ -425,25 +475,26 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
         }
         break;  // one tile a cluster; the sums are added up below
       }
-      const int ch = o.c0 + cl;
-      const bool on = ch < a.n;
-      const float sw = on ? __ldg(a.ws + (size_t)o.g * a.n + ch) : 0.f;
-      const float bias = on && a.bias ? __ldg(a.bias + (size_t)o.g * a.n + ch) : 0.f;
       T *out = reinterpret_cast<T *>(a.out) + (size_t)o.r0 * a.ld_out + ch;
-      for (int c = 0; c < o.nn; c += 16) {
-        uint32_t v[16];
+      for (int c = 0; c < o.nn; c += 32) {
+        uint32_t v[32];
+        // (the columns from c + 16 are there if the tile has them: nt is a multiple
+        // of 16, an accumulator a power of two)
         if (ok) {
           tc::ld16(tl + c, v);
+          if (c + 16 < o.nn) tc::ld16(tl + c + 16, v + 16);
           tc::wait_ld();
         }
-        const float sx = c + (lane & 15) < o.nn ? __ldg(a.xs + o.r0 + c + (lane & 15)) : 0.f;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float s = __shfl_sync(0xffffffffu, sx, j);
+        for (int j = 0; j < 32; ++j) {
+          const float s = __shfl_sync(0xffffffffu, xs[0], j);
           // a wait that ran out leaves NaN behind
           const float f = ok ? product_value((int)v[j], s, sw, bias) : __int_as_float(0x7fffffff);
-          if (on && c + j < o.nn) out[(size_t)(c + j) * a.ld_out] = ToF32<T>::put(f);
+          if (on && c + j < o.nn) *out = ToF32<T>::put(f);
+          out += a.ld_out;
         }
+#pragma unroll
+        for (int i = 0; i < 7; ++i) xs[i] = xs[i + 1];
       }
       tc::fence_before();
       __syncwarp();
@@ -454,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const GemmArgs a, con
     if (warp <= kMmaWarp) cluster_wait();
     // what the sums will be scaled by, loaded while they are on their way: a
     // thread keeps one channel of this CTA's own
-    const Tile o = tile0 < n_tiles ? tile_of(tile0, a, s_pre, s_off, ct) : Tile{0, 0, 0, 0};
+    const Tile o = tile0 < n_tiles ? tile_of<MB>(tile0, a, s_pre, s_off, ct) : Tile{0, 0, 0, 0};
     const int own = kM / a.cs, c = tid % own, ch = o.c0 + (int)rank * own + c, step = kThreads / own;
     const bool on = ch < a.n && tid < step * own;
     const float sw = on ? __ldg(a.ws + (size_t)o.g * a.n + ch) : 0.f;
@@ -657,11 +708,11 @@ int encode(CUtensorMap *m, const void *p, size_t rows, size_t k, size_t ld, int 
   return 0;
 }
 
-template <typename T>
+template <typename T, int MB>
 int launch_gemm(const GemmArgs &a, int grid, size_t smem, const Maps &maps, int dev, cudaStream_t st) {
   static bool attr[64] = {false};
   if (!attr[dev]) {
-    FFN_CUDA_TRY(cudaFuncSetAttribute(gemm_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax));
+    FFN_CUDA_TRY(cudaFuncSetAttribute(gemm_kernel<T, MB>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax));
     attr[dev] = true;
   }
   cudaLaunchAttribute at[2];
@@ -672,13 +723,13 @@ int launch_gemm(const GemmArgs &a, int grid, size_t smem, const Maps &maps, int 
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads_of(MB));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = at;
   cfg.numAttrs = a.cs > 1 ? 2 : 1;
   prof_begin(FFN_B200_K_INT8_GEMM, st);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_kernel<T>, a, maps);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_kernel<T, MB>, a, maps);
   prof_end(FFN_B200_K_INT8_GEMM, st);
   note_launch();
   if (e != cudaSuccess) {
@@ -694,6 +745,7 @@ struct GemmPlan {
   Maps maps;
   size_t smem;
   int grid, dev;
+  int mb;  // blocks of 128 channels a tile
 };
 int plan_gemm(GemmPlan &p, size_t rows, size_t n, size_t k, size_t n_groups, const int32_t *offsets, const int8_t *x,
               size_t ld_x, const float *x_scales, const int8_t *w, size_t ld_w, const float *w_scales, const float *bias,
@@ -723,42 +775,51 @@ int plan_gemm(GemmPlan &p, size_t rows, size_t n, size_t k, size_t n_groups, con
   a.rows = (int)rows, a.n = (int)n, a.groups = (int)n_groups;
   a.kt = (int)((k + kKB - 1) / kKB);
   a.kfull = (int)(k / kKB);
-  const long long ct = (long long)((n + kM - 1) / kM);
+  const long long ct1 = (long long)((n + kM - 1) / kM), ct2 = (long long)((n + 2 * kM - 1) / (2 * kM));
   a.cs = 1;
+  p.mb = 1;
   if (offsets) {
     // Groups: bound by the weights' bytes, so one chunk should hold a group: the
-    // average and three deviations of an even routing (48 experts of 8 rows each:
-    // 122 us with 32 rows a tile, 125 with 16).
+    // average and three deviations of an even routing (48 experts, K 2048, 128 rows
+    // each: 85 us with 160 rows a tile, 93 with 256, 94 with 128).  Two blocks of
+    // channels only for full tiles of 256 rows (512 rows each: 373 us, 435 with
+    // one; 128 rows each: 92 with two).
     const double avg = (double)rows / n_groups, want = avg + 3 * sqrt(avg);
-    a.nt = want <= 16 ? 16 : want >= 256 ? 256 : ((int)ceil(want) + 31) / 32 * 32;
+    a.nt = want >= 256 ? 256 : std::max(16, ((int)ceil(want) + 15) / 16 * 16);
+    if (want > 256 && n > (size_t)kM) p.mb = 2;
   } else {
-    // One matrix: the cheapest tile by waves x blocks of K x time a block (0.10 +
-    // 0.0029 us a token, measured at 4096 x 4096; 77 rows x 5120 x 2304: 9.5 us with
-    // 16 rows a tile, 11.5 with 32, 12.9 with 48).  K split over a cluster costs
+    // One matrix: the cheapest tile by waves x blocks of K x time a block, in us as
+    // measured at 4096 x 4096 (77 rows x 5120 x 2304: 9.5 us with 16 rows a tile,
+    // 11.5 with 32, 12.9 with 48; 8192 rows: 101 us with 256 x 224 tiles, four full
+    // waves, 106 with 256 x 256, 144 with 128 x 256).  K split over a cluster costs
     // 3.5 us more than it saves in blocks, and pays for few channels and a long K
     // (16 x 8192 x 1024: 7.9 us, 11.9 without).
     double best = 1e300;
-    for (int nt : {16, 32, 48, 64, 96, 128, 192, 256}) {
-      const long long chunks = (long long)((rows + nt - 1) / nt), tiles = ct * chunks;
-      const long long per = ((long long)rows + chunks - 1) / chunks, n16 = (per + 15) / 16 * 16;
-      const double block = 0.10 + 0.0029 * (double)n16;
+    for (int nt = 16; nt <= 256; nt += 16) {
+      const long long chunks = (long long)((rows + nt - 1) / nt), tiles = ct1 * chunks;
+      const double n16 = (double)((((long long)rows + chunks - 1) / chunks + 15) / 16 * 16);
+      const double block = std::min(0.10 + 0.0029 * n16, 0.30 + 0.00125 * n16);
       for (int cs = 1; cs <= 8; cs *= 2) {
         // (clusters that are sure to be resident at once)
         if (cs > 1 && (nt > kSplitRows || tiles * cs > sms * 3 / 4 || a.kt < 4 * cs)) break;
-        const double us = cs == 1 ? ceil((double)tiles / sms) * a.kt * block
-                                  : ceil((double)a.kt / cs) * block + 3.5 + 0.02 * (double)n16;
-        if (us < best) best = us, a.nt = nt, a.cs = cs;
+        const double us = cs == 1 ? ceil((double)tiles / sms) * a.kt * block : ceil((double)a.kt / cs) * block + 3.5 + 0.02 * n16;
+        if (us < best) best = us, a.nt = nt, a.cs = cs, p.mb = 1;
+      }
+      if (nt >= 128 && n > (size_t)kM) {
+        const double us = ceil((double)(ct2 * chunks) / sms) * (a.kt * (0.28 + 0.0021 * n16) + 1.0);
+        if (us < best) best = us, a.nt = nt, a.cs = 1, p.mb = 2;
       }
       if ((size_t)nt >= rows) break;
     }
   }
+  const long long ct = p.mb == 2 ? ct2 : ct1;
   // tiles at most: each group may end in a partial chunk
   const long long chunks = offsets ? std::min<long long>(rows, rows / a.nt + n_groups) : (rows + a.nt - 1) / a.nt;
   const long long tiles = ct * chunks;
   // (the kernel's tile numbers stay in 32 bits even where offsets are not ascending)
   if ((double)(rows / a.nt + 1) * (double)n_groups * (double)ct > 2147483647.0) return fail(FFN_B200_EINVAL, "int8_matmul: too many tiles");
   const size_t tail = (a.cs > 1 ? (size_t)kM * a.nt * 4 : 0) + (3 * n_groups + 1) * sizeof(int);
-  const size_t block = (size_t)kABytes + (size_t)a.nt * kKB, room = kSmemMax - 1024 - tail;
+  const size_t block = (size_t)p.mb * kABytes + (size_t)a.nt * kKB, room = kSmemMax - 1024 - tail;
   // as many blocks a stage, up to 4, as leave three stages: each costs its threads
   // a wait and a commit (64 blocks, 16 rows: 12.1 us with 4 a stage, 18.9 with 1),
   // and DRAM likes the rows' bytes together
@@ -769,38 +830,60 @@ int plan_gemm(GemmPlan &p, size_t rows, size_t n, size_t k, size_t n_groups, con
   if (a.stages < 2) return fail(FFN_B200_EUNSUP, "int8_matmul: too many groups for shared memory");
   p.smem = 1024 + a.stages * stage + tail;
   if (a.kfull) {
-    if (int rc = encode(&p.maps.w3, w, n_groups * n, k, ld_w, kM, a.sub)) return rc;
+    if (int rc = encode(&p.maps.w3, w, n_groups * n, k, ld_w, p.mb * kM, a.sub)) return rc;
     if (int rc = encode(&p.maps.x3, x, rows, k, ld_x, a.nt, a.sub)) return rc;
   }
   if (a.kfull < a.kt) {
-    if (int rc = encode(&p.maps.w2, w, n_groups * n, k, ld_w, kM, 0)) return rc;
+    if (int rc = encode(&p.maps.w2, w, n_groups * n, k, ld_w, p.mb * kM, 0)) return rc;
     if (int rc = encode(&p.maps.x2, x, rows, k, ld_x, a.nt, 0)) return rc;
   }
   p.grid = a.cs > 1 ? (int)tiles * a.cs : (int)std::min<long long>(tiles, sms);
   return 0;
 }
+template <typename T>
+int run_gemm_as(const GemmPlan &p, cudaStream_t st) {
+  return p.mb == 2 ? launch_gemm<T, 2>(p.a, p.grid, p.smem, p.maps, p.dev, st)
+                   : launch_gemm<T, 1>(p.a, p.grid, p.smem, p.maps, p.dev, st);
+}
 int run_gemm(const GemmPlan &p, int32_t dtype, cudaStream_t st) {
-  if (dtype == FFN_B200_DT_F32) return launch_gemm<float>(p.a, p.grid, p.smem, p.maps, p.dev, st);
-  if (dtype == FFN_B200_DT_BF16) return launch_gemm<__nv_bfloat16>(p.a, p.grid, p.smem, p.maps, p.dev, st);
-  return launch_gemm<__half>(p.a, p.grid, p.smem, p.maps, p.dev, st);
+  if (dtype == FFN_B200_DT_F32) return run_gemm_as<float>(p, st);
+  if (dtype == FFN_B200_DT_BF16) return run_gemm_as<__nv_bfloat16>(p, st);
+  return run_gemm_as<__half>(p, st);
 }
 
+template <typename T, int VEC, int MT, bool SWIGLU>
+int launch_quant_as(QuantArgs &a, cudaStream_t st) {
+  constexpr int NV = 16 / VEC;
+  constexpr size_t kStage = (size_t)kQuantStages * (SWIGLU ? 2 : 1) * NV * 16;  // bytes a thread
+  constexpr bool STAGED = VEC > 1 && kStage * MT <= (size_t)kSmemMax;
+  const int threads = (int)((a.n_vec + 32 * NV - 1) / (32 * NV) * 32);
+  int dev = 0;
+  FFN_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return fail(FFN_B200_EUNSUP, "quantize_int8: device index >= 64");
+  const size_t smem = STAGED ? kStage * threads : 0;
+  static bool attr[64] = {false};
+  if (STAGED && !attr[dev]) {
+    FFN_CUDA_TRY(cudaFuncSetAttribute(quant_kernel<T, VEC, NV, MT, SWIGLU, STAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)(kStage * MT)));
+    attr[dev] = true;
+  }
+  static int resident[64][MT / 32 + 1] = {{0}};
+  int &per_sm = resident[dev][threads / 32];
+  if (per_sm == 0) {
+    int n = 0;
+    FFN_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, quant_kernel<T, VEC, NV, MT, SWIGLU, STAGED>, threads, smem));
+    per_sm = std::max(1, n);
+  }
+  const int grid = (int)std::min<long long>(a.rows, (long long)sm_count_of(dev) * per_sm);
+  FFN_LAUNCH_PDL(FFN_B200_K_INT8_QUANT, st, "quantize_int8", (quant_kernel<T, VEC, NV, MT, SWIGLU, STAGED>), grid, threads, smem, a);
+  return 0;
+}
 template <typename T, int VEC, bool SWIGLU>
 int launch_quant(QuantArgs &a, cudaStream_t st) {
   a.n_vec = a.cols / VEC;
-#define FFN_GO(NV, W, GRID, THREADS) \
-  FFN_LAUNCH_PDL(FFN_B200_K_INT8_QUANT, st, "quantize_int8", (quant_kernel<T, VEC, NV, W, SWIGLU>), GRID, THREADS, 0, a)
-  // short rows a warp each, longer ones a CTA of just enough threads
-  if constexpr (VEC > 1) {
-    if (a.n_vec <= 128) FFN_GO(4, true, (a.rows + 7) / 8, 256);
-    else if (a.n_vec <= 2048) FFN_GO(2, false, a.rows, (int)((a.n_vec + 63) / 64 * 32));
-    else FFN_GO(4, false, a.rows, (int)((a.n_vec + 127) / 128 * 32));
-  } else {
-    if (a.n_vec <= 512) FFN_GO(16, true, (a.rows + 7) / 8, 256);
-    else FFN_GO(16, false, a.rows, (int)((a.n_vec + 511) / 512 * 32));
-  }
-#undef FFN_GO
-  return 0;
+  if (a.cols <= 4096) return launch_quant_as<T, VEC, 256, SWIGLU>(a, st);
+  if (a.cols <= 8192) return launch_quant_as<T, VEC, 512, SWIGLU>(a, st);
+  return launch_quant_as<T, VEC, 1024, SWIGLU>(a, st);
 }
 template <typename T, int VEC>
 int launch_quant_act(QuantArgs &a, int act, cudaStream_t st) {
