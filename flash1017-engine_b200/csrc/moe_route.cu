@@ -276,14 +276,16 @@ __global__ void __launch_bounds__(256) permute_kernel(const uint8_t *x, size_t l
 // DRAM-bound by the experts' rows, so what counts is loads on their way: with 6
 // ahead 64 registers are enough and 1024 threads an SM fit (8 ahead and 768
 // threads: 24576 rows of 4096 bf16 took 68 us, 3.4 TB/s).
+// Single elements (VEC 1) go four to a thread, so that looking a row up is not
+// most of the instructions (8192 x 6 x 4095 bf16: 501 us with one, 165 us).
 template <typename T, int VEC, int AHEAD>
 __global__ void __launch_bounds__(256, AHEAD > 6 ? 3 : 4) combine_rows_kernel(const T *y, size_t ld_y, uint32_t y_rows, const int32_t *pos,
                                                               const float *w, const T *residual, size_t ld_r, T *out,
                                                               size_t ld_o, int n_tok, int top_k, uint32_t n_vec, int tpt) {
+  constexpr int P = VEC == 1 ? 4 : 1;
   pdl_enter();
   const int l = threadIdx.x & (tpt - 1), per = 256 / tpt, lane = threadIdx.x & 31;
-  const uint32_t v = blockIdx.y * (uint32_t)tpt + l;
-  const bool on = v < n_vec;
+  const uint32_t v0 = blockIdx.y * (uint32_t)(tpt * P) + l;
   const long long step = (long long)gridDim.x * per;
   long long t = (long long)blockIdx.x * per + threadIdx.x / tpt;
   auto lookup = [&](long long tok, int k) { return tok < n_tok && k < top_k ? __ldg(pos + (size_t)tok * top_k + k) : -1; };
@@ -295,42 +297,56 @@ __global__ void __launch_bounds__(256, AHEAD > 6 ? 3 : 4) combine_rows_kernel(co
     float wl = next_w;
     next = lookup(t + step, lane);
     next_w = weight(t + step, lane);
-    Raw<T, VEC> rr = {};
-    if (residual && on) rr = load_raw<T, VEC>(residual + (size_t)t * ld_r, v);
-    float acc[VEC];
+    Raw<T, VEC> rr[P] = {};
+    if (residual)
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+      for (int i = 0; i < P; ++i)
+        if (v0 + i * tpt < n_vec) rr[i] = load_raw<T, VEC>(residual + (size_t)t * ld_r, v0 + i * tpt);
+    float acc[P][VEC];
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) acc[i][j] = 0.f;
     for (int k0 = 0; k0 < top_k; k0 += AHEAD) {
       if (k0 && (k0 & 31) == 0) pl = lookup(t, k0 + lane), wl = weight(t, k0 + lane);
-      Raw<T, VEC> r[AHEAD];
+      Raw<T, VEC> r[AHEAD][P];
       uint32_t use = 0;
 #pragma unroll
       for (int q = 0; q < AHEAD; ++q) {
         const uint32_t p = (uint32_t)__shfl_sync(0xffffffffu, pl, (k0 + q) & 31);
         if (k0 + q < top_k && p < y_rows) {
           use |= 1u << q;
-          if (on) r[q] = load_raw<T, VEC>(y + (size_t)p * ld_y, v);
+          const T *row = y + (size_t)p * ld_y;
+#pragma unroll
+          for (int i = 0; i < P; ++i)
+            if (v0 + i * tpt < n_vec) r[q][i] = load_raw<T, VEC>(row, v0 + i * tpt);
         }
       }
 #pragma unroll
       for (int q = 0; q < AHEAD; ++q) {
         const float f = __shfl_sync(0xffffffffu, wl, (k0 + q) & 31);
-        if (on && (use >> q & 1u)) {
-          float e[VEC];
-          unpack<T, VEC>(r[q], e);
+        if (use >> q & 1u)
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) acc[j] = fmaf(f, e[j], acc[j]);
-        }
+          for (int i = 0; i < P; ++i)
+            if (v0 + i * tpt < n_vec) {
+              float e[VEC];
+              unpack<T, VEC>(r[q][i], e);
+#pragma unroll
+              for (int j = 0; j < VEC; ++j) acc[i][j] = fmaf(f, e[j], acc[i][j]);
+            }
       }
     }
-    if (!on) continue;
-    if (residual) {
-      float e[VEC];
-      unpack<T, VEC>(rr, e);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) acc[j] += e[j];
+    for (int i = 0; i < P; ++i) {
+      if (v0 + i * tpt >= n_vec) continue;
+      if (residual) {
+        float e[VEC];
+        unpack<T, VEC>(rr[i], e);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[i][j] += e[j];
+      }
+      store_vec<T, VEC>(out + (size_t)t * ld_o, v0 + i * tpt, acc[i]);
     }
-    store_vec<T, VEC>(out + (size_t)t * ld_o, v, acc);
   }
 }
 
@@ -345,7 +361,7 @@ template <typename T, int VEC, int TPT>
 __global__ void __launch_bounds__(256, 3) combine_bwd_kernel(const T *dout, size_t ld_d, const T *y, size_t ld_y,
                                                           uint32_t y_rows, const int32_t *pos, const float *w, T *dy,
                                                           size_t ld_dy, float *dw, int n_tok, int top_k, uint32_t n_vec) {
-  constexpr int kTok = 256 / TPT;
+  constexpr int kTok = 256 / TPT, P = VEC == 1 ? 4 : 1;  // single elements four to a thread
   __shared__ float s_red[2][8][kBack];
   pdl_enter();
   const int l = threadIdx.x % TPT, lane = threadIdx.x & 31;
@@ -373,34 +389,44 @@ __global__ void __launch_bounds__(256, 3) combine_bwd_kernel(const T *dout, size
         f[q] = __shfl_sync(0xffffffffu, wl, (k0 + q) & 31);
         dot[q] = 0.f;
       }
-      for (uint32_t v = l; v < n_vec; v += TPT) {
-        Raw<T, VEC> r[kBack];
+      for (uint32_t v = l; v < n_vec; v += TPT * P) {
+        Raw<T, VEC> r[kBack][P], rd[P] = {};
         if (dw) {
 #pragma unroll
           for (int q = 0; q < kBack; ++q)
-            if (p[q] != 0xffffffffu) r[q] = load_raw<T, VEC>(y + (size_t)p[q] * ld_y, v);
+            if (p[q] != 0xffffffffu)
+#pragma unroll
+              for (int i = 0; i < P; ++i)
+                if (v + i * TPT < n_vec) r[q][i] = load_raw<T, VEC>(y + (size_t)p[q] * ld_y, v + i * TPT);
         }
-        float d[VEC];
-        unpack<T, VEC>(load_raw<T, VEC>(drow, v), d);
-        if (dy) {
 #pragma unroll
-          for (int q = 0; q < kBack; ++q)
-            if (p[q] != 0xffffffffu) {
-              float e[VEC];
+        for (int i = 0; i < P; ++i)
+          if (v + i * TPT < n_vec) rd[i] = load_raw<T, VEC>(drow, v + i * TPT);
 #pragma unroll
-              for (int j = 0; j < VEC; ++j) e[j] = f[q] * d[j];
-              store_vec<T, VEC>(dy + (size_t)p[q] * ld_dy, v, e);
-            }
-        }
-        if (dw) {
+        for (int i = 0; i < P; ++i) {
+          if (v + i * TPT >= n_vec) continue;
+          float d[VEC];
+          unpack<T, VEC>(rd[i], d);
+          if (dy) {
 #pragma unroll
-          for (int q = 0; q < kBack; ++q)
-            if (p[q] != 0xffffffffu) {
-              float e[VEC];
-              unpack<T, VEC>(r[q], e);
+            for (int q = 0; q < kBack; ++q)
+              if (p[q] != 0xffffffffu) {
+                float e[VEC];
 #pragma unroll
-              for (int j = 0; j < VEC; ++j) dot[q] = fmaf(d[j], e[j], dot[q]);
-            }
+                for (int j = 0; j < VEC; ++j) e[j] = f[q] * d[j];
+                store_vec<T, VEC>(dy + (size_t)p[q] * ld_dy, v + i * TPT, e);
+              }
+          }
+          if (dw) {
+#pragma unroll
+            for (int q = 0; q < kBack; ++q)
+              if (p[q] != 0xffffffffu) {
+                float e[VEC];
+                unpack<T, VEC>(r[q][i], e);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) dot[q] = fmaf(d[j], e[j], dot[q]);
+              }
+          }
         }
       }
       if (dw) {
@@ -462,8 +488,9 @@ template <typename T, int VEC, int AHEAD>
 int launch_combine_as(const void *y, size_t ld_y, size_t y_rows, const int32_t *pos, const float *w, const void *res,
                       size_t ld_r, void *out, size_t ld_o, size_t n_tok, size_t top_k, size_t cols, cudaStream_t st) {
   const uint32_t n_vec = (uint32_t)(cols / VEC);
-  const int tpt = threads_per_token(n_vec, 1);
-  const uint32_t seg = (n_vec + tpt - 1) / tpt;
+  constexpr int P = VEC == 1 ? 4 : 1;
+  const int tpt = threads_per_token(n_vec, P);
+  const uint32_t seg = (n_vec + tpt * P - 1) / (tpt * P);
   if (seg > 65535) return fail(FFN_B200_EUNSUP, "moe_combine: row too long for its alignment");
   const dim3 grid(grid_of((long long)(n_tok + 256 / tpt - 1) / (256 / tpt), 32), seg);
   FFN_LAUNCH_PDL(FFN_B200_K_ROUTE, st, "combine_rows_kernel", (combine_rows_kernel<T, VEC, AHEAD>), grid, 256, 0, (const T *)y,
