@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(MT, MT == 256 ? 3 : MT == 384 ? 2 : 1) fwd_ker
     }
   }
   const float inv_n = 1.f / (float)a.cols;
-  float gate = a.gate_kind == FFN_B200_GATE_TOKEN ? __ldg(a.gate + blockIdx.x) : 1.f;  // the next row's
+  float gate = a.gate_kind == FFN_B200_GATE_TOKEN ? a.gate[blockIdx.x] : 1.f;  // the next row's
   int par = 0, stage = 0;
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, par ^= 1) {
     Raw<T, VEC> r[2][NV] = {};
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(MT, MT == 256 ? 3 : MT == 384 ? 2 : 1) fwd_ker
             if (l + i * L < a.n_vec) r[w][i] = load_raw<T, VEC>(src[w] + (size_t)row * ld[w], l + i * L);
     }
     float k = gate;
-    if (a.gate_kind == FFN_B200_GATE_TOKEN && row + gridDim.x < a.rows) gate = __ldg(a.gate + row + gridDim.x);
+    if (a.gate_kind == FFN_B200_GATE_TOKEN && row + gridDim.x < a.rows) gate = a.gate[row + gridDim.x];
     if (a.post_w) {
       float s = 0.f;
 #pragma unroll
@@ -220,7 +220,8 @@ struct BwdArgs {
 // shared memory, every thread its own pieces, so a thread waits for its own
 // copies alone.  Without that DRAM idled through both reductions, and with the
 // parameters and three sums re-read per row the instructions took longer than
-// the bytes (4093 x 5120 f32: 134 us; staged 129 us; as here see launch_bwd).
+// the bytes (4093 x 5120 f32: 108 us unstaged, 100 us like this; 8192 x 4096
+// bf16: 112 and 88 us).
 template <typename T, int VEC, int NV, int MT, bool STAGED>
 __global__ void __launch_bounds__(MT) bwd_kernel(const BwdArgs a) {
   __shared__ float4 s_red[2][32];
@@ -313,7 +314,7 @@ __global__ void __launch_bounds__(MT) bwd_kernel(const BwdArgs a) {
     const float r_y = a.post_w ? rsqrtf(fmaf(s.x, inv_n, a.eps)) : 1.f;
     const float r_h = a.src[3] ? rsqrtf(fmaf(s.y, inv_n, a.eps)) : 0.f;
     const float m_h = s.z * inv_n * r_h * r_h;
-    const float gt = a.gate_kind == FFN_B200_GATE_TOKEN && a.src[0] ? __ldg(a.gate + row) : 1.f;
+    const float gt = a.gate_kind == FFN_B200_GATE_TOKEN && a.src[0] ? a.gate[row] : 1.f;
     const float k_br = a.beta * gt * r_y;
     float v[NV][VEC], q = 0.f;
 #pragma unroll
@@ -399,7 +400,7 @@ __global__ void __launch_bounds__(1024) colsum_kernel(const ColArgs a) {
 // ------------------------------------------------------------------ launch
 // Forward: 8 columns a thread up to 1024 columns, else 16: a row's reductions
 // and addresses cost a thread about as many instructions as 8 columns do (8192 x
-// 4096 bf16: 57 us with 8, issue-bound; 45 us with 16).
+// 4096 bf16: 60 us with 8, 46 us with 16).
 template <typename T, int VEC, int NV, int MT>
 int launch_fwd_as(FwdArgs &a, cudaStream_t st) {
   constexpr bool STAGED = VEC > 1 && (size_t)kFwdStages * 2 * NV * MT * 16 <= 224 * 1024;
@@ -415,7 +416,7 @@ int launch_fwd_as(FwdArgs &a, cudaStream_t st) {
     attr[dev] = true;
   }
   // as many CTAs as are resident at once: one more, and a second wave of whole
-  // shares of the rows would follow
+  // shares of the rows would follow (8192 x 4096 bf16: 51 us with half a wave more)
   static int resident[64][MT / 32 + 1] = {{0}};
   int &per_sm = resident[dev][threads / 32];
   if (per_sm == 0) {

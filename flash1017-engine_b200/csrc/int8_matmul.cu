@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(MT) quant_kernel(const QuantArgs a) {
   pdl_enter();
   const uint32_t l = threadIdx.x, L = blockDim.x;
   const int lane = l & 31, warp = l >> 5, nw = L >> 5;
-  const int rows = a.n_rows ? min(a.rows, __ldg(a.n_rows)) : a.rows;
+  const int rows = a.n_rows ? min(a.rows, *a.n_rows) : a.rows;
   uint4 *st = reinterpret_cast<uint4 *>(s_dyn) + l;
   auto fetch = [&](int stage, long long row) {
     if (row < rows) {
@@ -133,8 +133,7 @@ __global__ void __launch_bounds__(MT) quant_kernel(const QuantArgs a) {
 // ----------------------------------------------------------------- product
 // Warp 0: TMA, one thread; warp 1: MMA, one thread; warps 2-5: epilogue.  The two
 // single threads set the pace, so they count stages and phases instead of
-// dividing: two divisions a stage cost more than its waits and copies together
-// (8192 x 4096 x 4096: 97 us with them, 94 us without).
+// dividing.
 constexpr int kMmaWarp = 1;
 __host__ __device__ constexpr int threads_of(int mb) { return 64 + 128 * mb; }  // four epilogue warps a block of channels
 constexpr int kM = 128;             // channels a block; a tile has one or two (MB)
@@ -290,9 +289,10 @@ __global__ void __launch_bounds__(threads_of(MB), 1) gemm_kernel(const GemmArgs 
   const bool split = MB == 1 && a.cs > 1;
   int *s_off = red + (split ? kM * a.nt : 0);                          // [groups][first, count]
   int *s_pre = s_off + 2 * a.groups;                                      // [groups + 1]
-  // two accumulators; one where a cluster has a single tile.  At most 64 columns
-  // then, so that every cluster CTA an SM can hold gets its own: clusters that
-  // waited for each other's TMEM on two SMs would wait for good.
+  // Two accumulators; one where a cluster has a single tile.  It has at most 128
+  // columns then (32 up to 32 tokens), and so much shared memory that the cluster
+  // CTAs an SM can hold all find theirs: clusters that waited for each other's
+  // TMEM on two SMs would wait for good.
   const int acc_cols = a.nt <= 16 ? 16 : 1 << (32 - __clz(a.nt - 1)), tmem_cols = split ? max(32, acc_cols) : 2 * acc_cols;
   const uint32_t rank = a.cs > 1 ? ctarank() : 0;
   const int ct = (a.n + MB * kM - 1) / (MB * kM);
@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(threads_of(MB), 1) gemm_kernel(const GemmArgs 
     int sum = 0;
     for (int g = g0; g < g1; ++g) {
       // bounds from the GPU: kept inside the rows whatever they hold
-      const int lo = min(max(__ldg(a.offsets + g), 0), a.rows), hi = min(max(__ldg(a.offsets + g + 1), lo), a.rows);
+      const int lo = min(max(a.offsets[g], 0), a.rows), hi = min(max(a.offsets[g + 1], lo), a.rows);
       s_off[2 * g] = lo;
       s_off[2 * g + 1] = hi - lo;
       s_pre[g] = sum;
@@ -368,10 +368,8 @@ __global__ void __launch_bounds__(threads_of(MB), 1) gemm_kernel(const GemmArgs 
         for (int k = k_lo; k < k_hi; k += a.sub) {
           if (!wait_bar(&empty[s], ph ^ 1, &s_err, 1)) { live = false; break; }
           uint8_t *sw = smem + s * stage_bytes, *sx = sw + a.sub * kWBytes;
-          // One copy for all blocks of a stage: a single thread issues them, and
-          // with a copy per block and per 32 tokens it was what the kernel waited
-          // for (8192 x 4096 x 4096: 145 us; one box of 128 tokens 124 us).  Blocks
-          // past the last full one read as zeros.
+          // One copy an operand for all blocks of a stage, as a single thread issues
+          // them.  Blocks past the last full one read as zeros.
           const bool tail = a.kfull < a.kt && k + a.sub > a.kfull;
           const int n = tail ? min(a.sub, k_hi - k) : a.sub;
           tc::bar_arrive_tx(&full[s], n * (kWBytes + x_bytes));
@@ -438,7 +436,7 @@ __global__ void __launch_bounds__(threads_of(MB), 1) gemm_kernel(const GemmArgs 
     }
     __syncwarp();
   } else {
-    // -------------------------------------------------- epilogue (4 warps)
+    // -------------------------------------------------- epilogue (4 MB warps)
     // the second four of MB = 2 take the second block of channels
     const int quarter = warp & 3, mi = (warp - kMmaWarp - 1) >> 2, cl = quarter * 32 + lane;
     int n = 0;
@@ -453,10 +451,10 @@ __global__ void __launch_bounds__(threads_of(MB), 1) gemm_kernel(const GemmArgs 
       float xs[8], sw = 0.f, bias = 0.f;
       if (!split) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) xs[i] = 32 * i + lane < o.nn ? __ldg(a.xs + o.r0 + 32 * i + lane) : 0.f;
+        for (int i = 0; i < 8; ++i) xs[i] = 32 * i + lane < o.nn ? a.xs[o.r0 + 32 * i + lane] : 0.f;
         if (on) {
-          sw = __ldg(a.ws + (size_t)o.g * a.n + ch);
-          if (a.bias) bias = __ldg(a.bias + (size_t)o.g * a.n + ch);
+          sw = a.ws[(size_t)o.g * a.n + ch];
+          if (a.bias) bias = a.bias[(size_t)o.g * a.n + ch];
         }
       }
       const bool ok = __any_sync(0xffffffffu, lane == 0 && wait_bar(&acc_full[b], (n / kBufs) & 1, &s_err, 4));
@@ -508,9 +506,9 @@ __global__ void __launch_bounds__(threads_of(MB), 1) gemm_kernel(const GemmArgs 
     const Tile o = tile0 < n_tiles ? tile_of<MB>(tile0, a, s_pre, s_off, ct) : Tile{0, 0, 0, 0};
     const int own = kM / a.cs, c = tid % own, ch = o.c0 + (int)rank * own + c, step = kThreads / own;
     const bool on = ch < a.n && tid < step * own;
-    const float sw = on ? __ldg(a.ws + (size_t)o.g * a.n + ch) : 0.f;
-    const float bias = on && a.bias ? __ldg(a.bias + (size_t)o.g * a.n + ch) : 0.f;
-    for (int i = tid; i < o.nn; i += kThreads) s_xs[i] = __ldg(a.xs + o.r0 + i);
+    const float sw = on ? a.ws[(size_t)o.g * a.n + ch] : 0.f;
+    const float bias = on && a.bias ? a.bias[(size_t)o.g * a.n + ch] : 0.f;
+    for (int i = tid; i < o.nn; i += kThreads) s_xs[i] = a.xs[o.r0 + i];
     __syncthreads();
     if (s_err && tid < a.cs) st_peer(&s_err, tid, 1);  // all CTAs of the cluster learn of it
     __syncwarp();
@@ -556,12 +554,12 @@ __host__ __device__ constexpr int few_pitch(int k) { return (k + 4095) / 4096 * 
 
 // 16 weights from column 16 p of a row (zeros past k)
 __device__ __forceinline__ uint4 few_piece(const int8_t *row, int p, int k) {
-  if (16 * p + 16 <= k) return ldg_stream(row + 16 * p);
+  if (16 * p + 16 <= k) return load_once(row + 16 * p);
   union { uint4 v; int8_t b[16]; } u;
   u.v = make_uint4(0, 0, 0, 0);
 #pragma unroll
   for (int i = 0; i < 16; ++i)
-    if (16 * p + i < k) u.b[i] = __ldg(row + 16 * p + i);
+    if (16 * p + i < k) u.b[i] = row[16 * p + i];
   return u.v;
 }
 
@@ -649,7 +647,7 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(const FewArgs a) {
       if (base + 4096 < a.k) load(c, base + 4096);
       else load(c + step, 0);
     }
-    const float sw = __ldg(a.ws + c), bias = a.bias ? __ldg(a.bias + c) : 0.f;
+    const float sw = a.ws[c], bias = a.bias ? a.bias[c] : 0.f;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int sum = __reduce_add_sync(0xffffffffu, acc[r]);
@@ -821,7 +819,8 @@ int plan_gemm(GemmPlan &p, size_t rows, size_t n, size_t k, size_t n_groups, con
   const size_t tail = (a.cs > 1 ? (size_t)kM * a.nt * 4 : 0) + (3 * n_groups + 1) * sizeof(int);
   const size_t block = (size_t)p.mb * kABytes + (size_t)a.nt * kKB, room = kSmemMax - 1024 - tail;
   // as many blocks a stage, up to 4, as leave three stages: each costs its threads
-  // a wait and a commit (64 blocks, 16 rows: 12.1 us with 4 a stage, 18.9 with 1),
+  // a wait and a commit (77 rows x 5120 x 2304 with its quantisation: 10.9 us, 14.8
+  // with one; no effect on 8192 x 4096 x 4096),
   // and DRAM likes the rows' bytes together
   a.sub = 4;
   while (a.sub > 1 && (3 * a.sub * block > room || a.kt < 2 * a.sub * a.cs)) --a.sub;

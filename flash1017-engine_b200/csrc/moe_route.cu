@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortArgs a)
       if (p + 32 * i + lane < p1) {
         // unsigned: ids below e_begin, and the top-k step's "no candidate"
         // 0x7fffffff, fall outside like those at or above the range's end
-        const uint32_t r = (uint32_t)__ldg(a.idx + p + 32 * i + lane) - (uint32_t)a.e_begin;
+        const uint32_t r = (uint32_t)a.idx[p + 32 * i + lane] - (uint32_t)a.e_begin;
         if (r < (uint32_t)a.n_local) e[i] = (int)r;
       }
     }
@@ -218,9 +218,9 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortArgs a)
 constexpr int kSrcPairs = 16384;
 __global__ void __launch_bounds__(256) src_kernel(const int32_t *pos, const int32_t *total, int32_t *src, int n_pairs) {
   pdl_enter();
-  const int n = __ldg(total);
+  const int n = *total;
   for (int p = blockIdx.x * 256 + threadIdx.x; p < n_pairs; p += gridDim.x * 256) {
-    const uint32_t r = (uint32_t)__ldg(pos + p);
+    const uint32_t r = (uint32_t)pos[p];
     if (r < (uint32_t)n_pairs) src[r] = p;
     if (p >= n) src[p] = -1;
   }
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(256) permute_kernel(const uint8_t *x, size_t l
   const uint32_t v0 = blockIdx.y * (uint32_t)(tpt * kPieces) + l;
   const long long step = (long long)gridDim.x * per;
   long long t = (long long)blockIdx.x * per + threadIdx.x / tpt;
-  auto lookup = [&](long long tok, int k) { return tok < n_tok && k < top_k ? __ldg(pos + (size_t)tok * top_k + k) : -1; };
+  auto lookup = [&](long long tok, int k) { return tok < n_tok && k < top_k ? pos[(size_t)tok * top_k + k] : -1; };
   int32_t next = lookup(t, lane);
   for (; t < n_tok; t += step) {
     int32_t pl = next;
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(256) permute_kernel(const uint8_t *x, size_t l
 #pragma unroll
     for (int i = 0; i < kPieces; ++i)
       if (v0 + i * tpt < n_vec) r[i] = xr[v0 + i * tpt];
-    const float s = x_scale && v0 == 0 ? __ldg(x_scale + t) : 0.f;
+    const float s = x_scale && v0 == 0 ? x_scale[t] : 0.f;
     for (int k = 0; k < top_k; ++k) {
       if (k && (k & 31) == 0) pl = lookup(t, k + lane);
       const uint32_t p = (uint32_t)__shfl_sync(0xffffffffu, pl, k & 31);
@@ -288,8 +288,8 @@ __global__ void __launch_bounds__(256, AHEAD > 6 ? 3 : 4) combine_rows_kernel(co
   const uint32_t v0 = blockIdx.y * (uint32_t)(tpt * P) + l;
   const long long step = (long long)gridDim.x * per;
   long long t = (long long)blockIdx.x * per + threadIdx.x / tpt;
-  auto lookup = [&](long long tok, int k) { return tok < n_tok && k < top_k ? __ldg(pos + (size_t)tok * top_k + k) : -1; };
-  auto weight = [&](long long tok, int k) { return w && tok < n_tok && k < top_k ? __ldg(w + (size_t)tok * top_k + k) : 1.f; };
+  auto lookup = [&](long long tok, int k) { return tok < n_tok && k < top_k ? pos[(size_t)tok * top_k + k] : -1; };
+  auto weight = [&](long long tok, int k) { return w && tok < n_tok && k < top_k ? w[(size_t)tok * top_k + k] : 1.f; };
   int32_t next = lookup(t, lane);
   float next_w = weight(t, lane);
   for (; t < n_tok; t += step) {
@@ -367,8 +367,8 @@ __global__ void __launch_bounds__(256, 3) combine_bwd_kernel(const T *dout, size
   const int l = threadIdx.x % TPT, lane = threadIdx.x & 31;
   const long long step = (long long)gridDim.x * kTok;
   long long t = (long long)blockIdx.x * kTok + threadIdx.x / TPT;
-  auto lookup = [&](long long tok, int k) { return tok < n_tok && k < top_k ? __ldg(pos + (size_t)tok * top_k + k) : -1; };
-  auto weight = [&](long long tok, int k) { return w && tok < n_tok && k < top_k ? __ldg(w + (size_t)tok * top_k + k) : 1.f; };
+  auto lookup = [&](long long tok, int k) { return tok < n_tok && k < top_k ? pos[(size_t)tok * top_k + k] : -1; };
+  auto weight = [&](long long tok, int k) { return w && tok < n_tok && k < top_k ? w[(size_t)tok * top_k + k] : 1.f; };
   int32_t next = lookup(t, lane);
   float next_w = weight(t, lane);
   int par = 0;

@@ -19,6 +19,16 @@ inline bool dtype_ok(int dt) {
   return dt == FFN_B200_DT_F32 || dt == FFN_B200_DT_BF16 || dt == FFN_B200_DT_F16;
 }
 
+// Loads here are plain ones.  Kernels start before the previous one has finished
+// (programmatic dependent launch) and may read what it writes, so the read-only
+// path, which wants data that nothing writes while the kernel runs, is not used.
+__device__ __forceinline__ uint4 load_once(const void *p) {  // not kept in L1
+  uint4 r;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p) : "memory");
+  return r;
+}
+
 template <int BYTES> struct RawOf;
 template <> struct RawOf<16> { using type = uint4; };
 template <> struct RawOf<8> { using type = uint2; };
@@ -77,12 +87,12 @@ __device__ __forceinline__ void load_param(const float *p, size_t vec, float (&f
   if constexpr (VEC % 4 == 0) {
 #pragma unroll
     for (int i = 0; i < VEC / 4; ++i) {
-      const float4 v = __ldg(reinterpret_cast<const float4 *>(p) + vec * (VEC / 4) + i);
+      const float4 v = reinterpret_cast<const float4 *>(p)[vec * (VEC / 4) + i];
       f[4 * i] = v.x, f[4 * i + 1] = v.y, f[4 * i + 2] = v.z, f[4 * i + 3] = v.w;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] = __ldg(p + vec * VEC + i);
+    for (int i = 0; i < VEC; ++i) f[i] = p[vec * VEC + i];
   }
 }
 

@@ -341,7 +341,7 @@ FFN_B200_EXPORT int ffn_b200_int8_matmul(size_t rows, size_t n, size_t k, size_t
                                          size_t ld_w, const float *w_scales, const float *bias, int32_t dtype,
                                          void *out, size_t ld_out, void *stream);
 /* quantize_int8 of float rows x (x_dtype, k <= 16384) and int8_matmul, in one call:
- * the same bits.  Up to 4 rows and one matrix take one launch and no workspace;
+ * the same bits.  One or two rows and one matrix take one launch and no workspace;
  * else ws (16-byte aligned, int8_linear_ws_bytes) holds the codes. */
 FFN_B200_EXPORT size_t ffn_b200_int8_linear_ws_bytes(size_t rows, size_t k, size_t n_groups,
                                                      const int32_t *offsets);
