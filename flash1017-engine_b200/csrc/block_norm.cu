@@ -526,6 +526,7 @@ int ffn_b200_block_norm(const ffn_b200_block_norm_desc *d, const void *y, size_t
   const size_t es = dtype_bytes(d->dtype);
   if (((uintptr_t)y | (uintptr_t)residual | (uintptr_t)h | (uintptr_t)xn) % es)
     return fail(FFN_B200_EINVAL, "block_norm: rows must be aligned to their type");
+  if ((uintptr_t)code_scales % 4) return fail(FFN_B200_EINVAL, "block_norm: code_scales must be 4-byte aligned");
   FwdArgs a{};
   a.y = y, a.res = residual, a.h = h, a.xn = xn, a.codes = codes, a.code_scale = code_scales;
   a.ld_y = ld_y, a.ld_r = ld_res, a.ld_h = ld_h, a.ld_x = ld_xn, a.ld_c = ld_codes;
@@ -564,6 +565,8 @@ int ffn_b200_block_norm_bwd(const ffn_b200_block_norm_desc *d, const void *y, si
   if (int rc = check_desc("block_norm_bwd", d)) return rc;
   if ((dpost_w && !d->post_w) || (dgate && !d->gate))
     return fail(FFN_B200_EINVAL, "block_norm_bwd: a gradient of a parameter that is not there");
+  if (((uintptr_t)dpost_w | (uintptr_t)dgate | (uintptr_t)dpre_w) % 4)
+    return fail(FFN_B200_EINVAL, "block_norm_bwd: parameter gradients must be 4-byte aligned");
   const bool chan = d->gate_kind == FFN_B200_GATE_CHANNEL && dgate;
   cudaStream_t st = (cudaStream_t)stream;
   if (d->rows == 0) {  // sums over no rows

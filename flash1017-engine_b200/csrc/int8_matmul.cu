@@ -290,9 +290,9 @@ __global__ void __launch_bounds__(threads_of(MB), 1) gemm_kernel(const GemmArgs 
   int *s_off = red + (split ? kM * a.nt : 0);                          // [groups][first, count]
   int *s_pre = s_off + 2 * a.groups;                                      // [groups + 1]
   // Two accumulators; one where a cluster has a single tile.  It has at most 128
-  // columns then (32 up to 32 tokens), and so much shared memory that the cluster
-  // CTAs an SM can hold all find theirs: clusters that waited for each other's
-  // TMEM on two SMs would wait for good.
+  // columns then (32 up to 32 tokens), and at least 175 KB of shared memory, so an
+  // SM holds one such CTA, of whatever stream: clusters that waited for each
+  // other's TMEM on two SMs would wait for good.
   const int acc_cols = a.nt <= 16 ? 16 : 1 << (32 - __clz(a.nt - 1)), tmem_cols = split ? max(32, acc_cols) : 2 * acc_cols;
   const uint32_t rank = a.cs > 1 ? ctarank() : 0;
   const int ct = (a.n + MB * kM - 1) / (MB * kM);
@@ -759,8 +759,9 @@ int plan_gemm(GemmPlan &p, size_t rows, size_t n, size_t k, size_t n_groups, con
   if (((uintptr_t)x | (uintptr_t)w | ld_x | ld_w) % 16)
     return fail(FFN_B200_EINVAL, "int8_matmul: x, w and their row strides must be multiples of 16 bytes");
   if (ld_x < k || ld_w < k || (rows > 1 && ld_out < n)) return fail(FFN_B200_EINVAL, "int8_matmul: rows overlap");
-  if ((uintptr_t)out % dtype_bytes(dtype) || ((uintptr_t)x_scales | (uintptr_t)w_scales | (uintptr_t)bias) % 4)
-    return fail(FFN_B200_EINVAL, "int8_matmul: out and scales must be aligned to their type");
+  if ((uintptr_t)out % dtype_bytes(dtype) ||
+      ((uintptr_t)x_scales | (uintptr_t)w_scales | (uintptr_t)bias | (uintptr_t)offsets) % 4)
+    return fail(FFN_B200_EINVAL, "int8_matmul: out, scales and offsets must be aligned to their type");
   FFN_CUDA_TRY(cudaGetDevice(&p.dev));
   const int dev = p.dev;
   if (dev < 0 || dev >= 64) return fail(FFN_B200_EUNSUP, "int8_matmul: device index >= 64");
@@ -907,8 +908,8 @@ int ffn_b200_quantize_int8(size_t rows, size_t cols, int32_t dtype, const void *
   if (!x || !codes || !scales) return fail(FFN_B200_EINVAL, "quantize_int8: null pointer");
   const size_t width = act == FFN_B200_ACT_SWIGLU ? 2 * cols : cols, es = dtype_bytes(dtype);
   if (rows > 1 && (ld_x < width || ld_codes < cols)) return fail(FFN_B200_EINVAL, "quantize_int8: rows overlap");
-  if ((uintptr_t)x % es || (uintptr_t)scales % 4)
-    return fail(FFN_B200_EINVAL, "quantize_int8: rows and scales must be aligned to their type");
+  if ((uintptr_t)x % es || ((uintptr_t)scales | (uintptr_t)n_rows) % 4)
+    return fail(FFN_B200_EINVAL, "quantize_int8: rows, scales and n_rows must be aligned to their type");
   QuantArgs a{};
   a.x = x, a.ld_x = ld_x, a.codes = codes, a.ld_c = ld_codes, a.scales = scales, a.n_rows = n_rows;
   a.rows = (int)rows, a.cols = (uint32_t)cols;

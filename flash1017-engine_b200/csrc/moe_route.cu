@@ -549,6 +549,8 @@ int ffn_b200_moe_sort(size_t n_tok, size_t top_k, const int32_t *idx, int32_t ex
   using namespace ffn::route;
   if (int rc = check_pairs("moe_sort", n_tok, top_k, 0)) return rc;
   if (!offsets || (n_tok && !idx)) return fail(FFN_B200_EINVAL, "moe_sort: null pointer");
+  if (((uintptr_t)idx | (uintptr_t)offsets | (uintptr_t)pos | (uintptr_t)src) % 4)
+    return fail(FFN_B200_EINVAL, "moe_sort: arrays must be 4-byte aligned");
   if (expert_begin < 0 || expert_end <= expert_begin || expert_end - expert_begin > 4096)
     return fail(FFN_B200_EINVAL, "moe_sort: the expert range must be 1..4096 experts from expert_begin >= 0");
   cudaStream_t st = (cudaStream_t)stream;
@@ -631,6 +633,8 @@ int ffn_b200_moe_permute(size_t n_tok, size_t top_k, size_t row_bytes, const voi
   if (!x || !pos || !out) return fail(FFN_B200_EINVAL, "moe_permute: null pointer");
   if ((x_scale == nullptr) != (out_scale == nullptr))
     return fail(FFN_B200_EINVAL, "moe_permute: x_scale and out_scale go together");
+  if (((uintptr_t)pos | (uintptr_t)x_scale | (uintptr_t)out_scale) % 4)
+    return fail(FFN_B200_EINVAL, "moe_permute: pos and scales must be 4-byte aligned");
   if (row_bytes == 0 || row_bytes > (1u << 30)) return fail(FFN_B200_EINVAL, "moe_permute: bad row size");
   if ((n_tok > 1 && ld_x < row_bytes) || (out_rows > 1 && ld_out < row_bytes))
     return fail(FFN_B200_EINVAL, "moe_permute: rows overlap");
@@ -656,6 +660,7 @@ int ffn_b200_moe_combine(size_t n_tok, size_t top_k, size_t cols, int32_t dtype,
   const size_t es = dtype_bytes(dtype);
   if (((uintptr_t)y | (uintptr_t)residual | (uintptr_t)out) % es)
     return fail(FFN_B200_EINVAL, "moe_combine: rows must be aligned to their type");
+  if (((uintptr_t)pos | (uintptr_t)w) % 4) return fail(FFN_B200_EINVAL, "moe_combine: pos and w must be 4-byte aligned");
   const bool v16 = cols * es % 16 == 0 && rows16(y, ld_y, es) && rows16(out, ld_out, es) && rows16(residual, ld_res, es);
   cudaStream_t st = (cudaStream_t)stream;
 #define FFN_CALL(T, V) launch_combine_rows<T, V>(y, ld_y, y_rows, pos, w, residual, ld_res, out, ld_out, n_tok, top_k, cols, st)
@@ -679,6 +684,8 @@ int ffn_b200_moe_combine_bwd(size_t n_tok, size_t top_k, size_t cols, int32_t dt
   const size_t es = dtype_bytes(dtype);
   if (((uintptr_t)y | (uintptr_t)dout | (uintptr_t)dy) % es)
     return fail(FFN_B200_EINVAL, "moe_combine_bwd: rows must be aligned to their type");
+  if (((uintptr_t)pos | (uintptr_t)w | (uintptr_t)dw) % 4)
+    return fail(FFN_B200_EINVAL, "moe_combine_bwd: pos, w and dw must be 4-byte aligned");
   const bool v16 = cols * es % 16 == 0 && rows16(dw ? y : nullptr, ld_y, es) && rows16(dout, ld_dout, es) && rows16(dy, ld_dy, es);
   cudaStream_t st = (cudaStream_t)stream;
 #define FFN_CALL(T, V) launch_combine_bwd<T, V>(dout, ld_dout, y, ld_y, y_rows, pos, w, dy, ld_dy, dw, n_tok, top_k, cols, st)

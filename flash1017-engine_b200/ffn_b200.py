@@ -1156,7 +1156,8 @@ def moe_combine_backward(dout, y, pos, weight=None, dy=None, stream=None):
     """Gradients of moe_combine: (dy, dw), dy[pos[t, k]] = weight[t, k] dout[t],
     dw [tokens, top_k] f32 (ffn_b200_moe_combine_bwd).  The residual's gradient
     is dout.  A new dy has zeros in the rows that no pair names; in a given one
-    they are left as they were."""
+    they are left as they were.  No two pairs may name the same row (moe_sort's
+    never do)."""
     dev = _dev(y, stream)
     if dev < 0:
         with _on(y, stream):

@@ -335,14 +335,15 @@ FFN_B200_EXPORT int ffn_b200_quantize_int8(size_t rows, size_t cols, int32_t dty
  * outside 0..rows are clamped); NULL: one group of all rows.  Rows in no group
  * are left as they were.  x, w 16-byte aligned, ld_x and ld_w multiples of 16;
  * any n and k (bytes of a row behind k are not used).  At most 4096 groups; no
- * workspace.  A wait inside the kernel that runs out writes NaN. */
+ * workspace; out must not overlap an input.  A wait inside the kernel that runs out writes NaN. */
 FFN_B200_EXPORT int ffn_b200_int8_matmul(size_t rows, size_t n, size_t k, size_t n_groups, const int32_t *offsets,
                                          const int8_t *x, size_t ld_x, const float *x_scales, const int8_t *w,
                                          size_t ld_w, const float *w_scales, const float *bias, int32_t dtype,
                                          void *out, size_t ld_out, void *stream);
 /* quantize_int8 of float rows x (x_dtype, k <= 16384) and int8_matmul, in one call:
  * the same bits.  One or two rows and one matrix take one launch and no workspace;
- * else ws (16-byte aligned, int8_linear_ws_bytes) holds the codes. */
+ * else ws (16-byte aligned, int8_linear_ws_bytes) holds the codes.  out and ws must
+ * overlap nothing; calls that may run at the same time need a ws each. */
 FFN_B200_EXPORT size_t ffn_b200_int8_linear_ws_bytes(size_t rows, size_t k, size_t n_groups,
                                                      const int32_t *offsets);
 FFN_B200_EXPORT int ffn_b200_int8_linear(size_t rows, size_t n, size_t k, size_t n_groups, const int32_t *offsets,
@@ -368,7 +369,8 @@ FFN_B200_EXPORT int ffn_b200_moe_sort(size_t n_tok, size_t top_k, const int32_t 
 /* out[pos[t][k]] = x[t]: rows of row_bytes bytes, ld_x and ld_out in BYTES, any
  * type; with x_scale [n_tok] also out_scale[pos[t][k]] = x_scale[t] (int8 rows and
  * their scales).  Pairs with pos outside [0, out_rows) are skipped, rows that no
- * pair names are left as they were.  out must not overlap x. */
+ * pair names are left as they were.  A row that two pairs name (none of moe_sort's
+ * is) gets one of them.  out must not overlap x. */
 FFN_B200_EXPORT int ffn_b200_moe_permute(size_t n_tok, size_t top_k, size_t row_bytes, const void *x,
                                          size_t ld_x, const int32_t *pos, size_t out_rows, void *out,
                                          size_t ld_out, const float *x_scale, float *out_scale, void *stream);
@@ -382,7 +384,9 @@ FFN_B200_EXPORT int ffn_b200_moe_combine(size_t n_tok, size_t top_k, size_t cols
 /* The gradient of moe_combine: dy[pos[t][k]] = w[t][k] * dout[t] (w NULL: 1) and
  * dw[t][k] = sum of dout[t] * y[pos[t][k]] (0 where pos is outside [0, y_rows));
  * either of dy, dw may be NULL, y too without dw.  Rows of dy that no pair names
- * are left as they were.  The residual's gradient is dout. */
+ * are left as they were, and no two pairs may name the same row (moe_sort's never
+ * do): its dy would be one of theirs, not their sum.  The residual's gradient is
+ * dout.  dy and dw must not overlap an input. */
 FFN_B200_EXPORT int ffn_b200_moe_combine_bwd(size_t n_tok, size_t top_k, size_t cols, int32_t dtype,
                                              const void *dout, size_t ld_dout, const void *y, size_t ld_y,
                                              size_t y_rows, const int32_t *pos, const float *w, void *dy,

@@ -170,3 +170,33 @@ def test_the_module_of_calls_is_built_and_leaves_what_it_does_not_take(ffn):
     assert m.moe_combine(x, i32, None, None) is None
     with pytest.raises(TypeError):
         m.moe_sort(i32, 0)
+
+
+def test_misaligned_side_arrays_are_refused(ffn):
+    """Indices, offsets, weights, scales and parameter gradients of 4 bytes: a
+    misaligned one is an error of the call, not of the GPU."""
+    L, M = ffn.lib(), P + 2
+    for at in (2, 5, 6, 7):
+        a = [4, 2, P, 0, 8, P, P, P]
+        a[at] = M
+        refused(ffn, L.ffn_b200_moe_sort(*a, None), EINVAL, b"4-byte")
+    for at in (5, 9, 10):
+        a = [4, 2, 64, P, 64, P, 8, P, 64, P, P]
+        a[at] = M
+        refused(ffn, L.ffn_b200_moe_permute(*a, None), EINVAL, b"4-byte")
+    for at in (7, 8):
+        a = [4, 2, 16, 0, P, 16, 8, P, P, None, 0, P, 16]
+        a[at] = M
+        refused(ffn, L.ffn_b200_moe_combine(*a, None), EINVAL, b"4-byte")
+    for at in (9, 10, 13):
+        a = [4, 2, 16, 0, P, 16, P, 16, 8, P, P, P, 16, P]
+        a[at] = M
+        refused(ffn, L.ffn_b200_moe_combine_bwd(*a, None), EINVAL, b"4-byte")
+    refused(ffn, product(ffn, offsets=M), EINVAL, b"aligned")
+    refused(ffn, L.ffn_b200_quantize_int8(4, 64, 1, P, 64, 0, M, P, 64, P, None), EINVAL, b"aligned")
+    refused(ffn, L.ffn_b200_block_norm(C.byref(desc(ffn)), P, 64, P, 64, P, 64, P, 64, P, 64, M, None), EINVAL, b"4-byte")
+    d = desc(ffn, kind=1, gate=P)
+    for at in (13, 14, 15):
+        a = [C.byref(d), P, 64, P, 64, P, 64, P, 64, P, 64, P, 64, None, None, None]
+        a[at] = M
+        refused(ffn, L.ffn_b200_block_norm_bwd(*a, P, 1 << 30, None), EINVAL, b"4-byte")
