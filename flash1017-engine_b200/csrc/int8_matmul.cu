@@ -47,10 +47,10 @@ __device__ __forceinline__ float swiglu10(float g, float u) {
 }
 
 // Persistent, a row per CTA at a time; thread l holds the columns of pieces l, l +
-// L, ... (16 in all) and has its pieces of the CTA's next two rows brought into
-// shared memory meanwhile (STAGED).  A CTA a row took 22 us for 8192 x 4096 bf16
-// (4.5 TB/s), 21 us like this.
-constexpr int kQuantStages = 3;
+// L, ... (16 in all) and has its pieces of the CTA's next row brought into shared
+// memory meanwhile (STAGED; a third stage costs resident CTAs: 8192 x 4096 f32 30.4
+// us, 28.0 with two).
+constexpr int kQuantStages = 2;
 template <typename T, int VEC, int NV, int MT, bool SWIGLU, bool STAGED>
 __global__ void __launch_bounds__(MT) quant_kernel(const QuantArgs a) {
   constexpr int W = SWIGLU ? 2 : 1;  // gate and up
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(MT) quant_kernel(const QuantArgs a) {
       __syncthreads();
       m = __reduce_max_sync(0xffffffffu, lane < nw ? s_red[par][lane] : 0u);
     }
-    const Int8Row sc(SWIGLU ? __uint_as_float(m) : from_abs_bits<T>(m));
+    const Int8Row sc = SWIGLU ? Int8Row(__uint_as_float(m)) : Int8Row::of_bits<T>(m);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (l + i * L >= a.n_vec) continue;
@@ -605,7 +605,7 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(const FewArgs a) {
   float scale[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const Int8Row sc(from_abs_bits<T>(__reduce_max_sync(0xffffffffu, lane < kWarps ? s_max[r][lane] : 0u)));
+    const Int8Row sc = Int8Row::of_bits<T>(__reduce_max_sync(0xffffffffu, lane < kWarps ? s_max[r][lane] : 0u));
     scale[r] = sc.scale();
     const T *x = (const T *)a.x + (size_t)r * a.ld_x;
     int8_t *q = s_codes + r * pitch;

@@ -93,3 +93,28 @@ def test_calls_on_several_streams_at_once(ffn, cuda):
     torch.cuda.synchronize()
     for outs in got:
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("dtype,bits,low", [("float16", 10, 0), ("float16", 10, -14), ("bfloat16", 7, 0), ("bfloat16", 7, -80),
+                                            ("bfloat16", 7, -100)])
+def test_codes_of_every_significand(ffn, cuda, dtype, bits, low):
+    """A row for every significand of the largest value, holding every value of
+    its type below it down to 2^-10 of it, in both signs: codes next to every
+    half, and on it.  f16 rows around 2^-14 reach its subnormals."""
+    import torch
+    dt = getattr(torch, dtype)
+    sig = torch.arange(1 << bits, 2 << bits, dtype=torch.float64)
+    m = sig * 2.0 ** (low - bits)
+    x = (sig[None, :] * 2.0 ** (low - bits)) * 2.0 ** -torch.arange(10, dtype=torch.float64)[:, None]
+    x = x.reshape(1, -1).expand(m.numel(), -1).clone()
+    x[x > m[:, None]] = 0.0
+    x[:, 1::2] *= -1
+    for flip in (1.0, -1.0):
+        rows = torch.cat([m[:, None], flip * x], 1).to(dt)
+        for take in (rows, rows[:, :-(rows.shape[1] % 8)]):  # single elements, and 16 bytes at a time
+            take = take.contiguous()
+            q, s = ffn.quantize_int8(take.to(cuda))
+            # tensor by tensor: IEEE division in f32, ties to even
+            scale = take.float().abs().amax(1) / torch.full((len(take),), 127.0)
+            want = torch.round(take.float() / scale[:, None])
+            assert torch.equal(s.cpu(), scale) and torch.equal(q.cpu().float(), want)
