@@ -24,9 +24,8 @@ namespace route {
 // contiguous segment of the pairs.  A warp ranks 32 pairs at a time (the lanes
 // with the same expert, found by a ballot per bit of the expert number, in lane
 // order), so the order inside an expert is the pair order.  match.any finds the
-// same lanes in one instruction, but its latency was most of the kernel's time
-// (49152 pairs: 20 us).  Counts per (segment, expert) sit in shared
-// memory; the CTAs of the cluster read each other's totals over distributed
+// same lanes in one instruction, but its latency was most of the kernel's time.
+// Counts per (segment, expert) sit in shared memory; the CTAs of the cluster read each other's totals over distributed
 // shared memory, which saves the second and third launch and the workspace
 // that a grid-wide sort would need.  Bound by latency, not by bytes: 8 bytes
 // a pair.
@@ -83,7 +82,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortArgs a)
   const uint32_t rank = cluster_rank(), nrank = cluster_size();
   int *tot = s_cnt + a.segs * a.n_local, *off = tot + a.n_local;
   // pass 1: counts per segment.  kSortBatch groups of ids are asked for before the
-  // first is ranked (one at a time, 49152 pairs took 15 us, most of it latency).
+  // first is ranked: one at a time, their latency was most of the time.
   const long long s0 = ((long long)rank * a.segs + warp) * a.per_seg;
   const int p0 = (int)min(s0, (long long)a.n_pairs), p1 = (int)min(s0 + a.per_seg, (long long)a.n_pairs);
   int *mine = s_cnt + warp * a.n_local;
@@ -275,7 +274,7 @@ __global__ void __launch_bounds__(256) permute_kernel(const uint8_t *x, size_t l
 // A thread's piece of AHEAD routed rows is loaded before the first is used.
 // DRAM-bound by the experts' rows, so what counts is loads on their way: with 6
 // ahead 64 registers are enough and 1024 threads an SM fit (8 ahead and 768
-// threads: 24576 rows of 4096 bf16 took 68 us, 3.4 TB/s).
+// threads: 24576 rows of 4096 bf16 take 61 us, like this 52).
 // Single elements (VEC 1) go four to a thread, so that looking a row up is not
 // most of the instructions (8192 x 6 x 4095 bf16: 501 us with one, 165 us).
 template <typename T, int VEC, int AHEAD>
@@ -567,7 +566,7 @@ int ffn_b200_moe_sort(size_t n_tok, size_t top_k, const int32_t *idx, int32_t ex
   const bool later = src && pos && a.n_pairs > kSrcPairs;
   a.src = later ? nullptr : src;
   // One CTA up to 512 pairs (384 experts: 4.5 us for 384 pairs, but 7.3 us for 2046
-  // against 4.8 us with the cluster).
+  // against 4.5 us with the cluster).
   // Above 8192 pairs 16 CTAs (49152 pairs: 11.0 us with 8, 9.8 us), where this
   // GPU can hold such a cluster.
   static int widest[64] = {0};
