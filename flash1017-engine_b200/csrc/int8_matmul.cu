@@ -292,7 +292,9 @@ __global__ void __launch_bounds__(threads_of(MB), 1) gemm_kernel(const GemmArgs 
   // Two accumulators; one where a cluster has a single tile.  It has at most 128
   // columns then (32 up to 32 tokens), and at least 175 KB of shared memory, so an
   // SM holds one such CTA, of whatever stream: clusters that waited for each
-  // other's TMEM on two SMs would wait for good.
+  // other's TMEM on two SMs would wait for good.  Other CTAs may share an SM (a K of
+  // 256 in tiles of 256 tokens is 97 KB, but all of TMEM), and the allocation then
+  // waits for the other's, of whatever stream.
   const int acc_cols = a.nt <= 16 ? 16 : 1 << (32 - __clz(a.nt - 1)), tmem_cols = split ? max(32, acc_cols) : 2 * acc_cols;
   const uint32_t rank = a.cs > 1 ? ctarank() : 0;
   const int ct = (a.n + MB * kM - 1) / (MB * kM);
@@ -308,7 +310,6 @@ __global__ void __launch_bounds__(threads_of(MB), 1) gemm_kernel(const GemmArgs 
       asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.x3) : "memory");
     }
   }
-  if (warp == kMmaWarp) tc::alloc(&s_tmem, tmem_cols);
   const int k_lo = split ? a.kt * (int)rank / a.cs : 0, k_hi = split ? a.kt * ((int)rank + 1) / a.cs : a.kt;
   const int tile0 = (int)(blockIdx.x / a.cs), tile_step = (int)(gridDim.x / a.cs);
   if (!a.offsets && warp == 0 && lane < a.stages && k_lo + lane * a.sub < min(k_hi, a.kfull)) {
@@ -319,6 +320,10 @@ __global__ void __launch_bounds__(threads_of(MB), 1) gemm_kernel(const GemmArgs 
       tma_prefetch_l2(&maps.w3, tile0 / chunks * MB * kM, k_lo + lane * a.sub);
   }
   pdl_enter();
+  // Behind the wait for the previous kernel: whoever holds TMEM depends on nothing
+  // but its own work.  A CTA that held it while it waited could hold what a CTA of
+  // that previous kernel is still waiting for, itself or through another stream's.
+  if (warp == kMmaWarp) tc::alloc(&s_tmem, tmem_cols);
 
   // token chunks of each group
   if (a.offsets) {
