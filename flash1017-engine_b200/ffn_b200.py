@@ -988,7 +988,10 @@ class Int8Matrix:
         output channel (ffn_b200_quantize_int8 over the channels)."""
         if w.dim() not in (2, 3):
             raise FfnError("Int8Matrix.quantize: w must be [rows, cols] or [groups, rows, cols]")
-        codes, scales = quantize_int8(w.reshape(-1, w.shape[-1]), stream=stream)
+        if _dev(w, stream) < 0:
+            with _on(w, stream):  # reshape copies: on the kernel's stream, in its memory
+                return cls.quantize(w, bias)
+        codes, scales = quantize_int8(w.reshape(-1, w.shape[-1]))
         ld = (w.shape[-1] + 15) // 16 * 16
         codes = codes.as_strided(w.shape, ((w.shape[1] * ld, ld, 1) if w.dim() == 3 else (ld, 1)))
         return cls(codes, scales, bias)

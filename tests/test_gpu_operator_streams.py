@@ -35,3 +35,25 @@ def test_products_of_short_k_behind_each_other_on_several_streams(ffn, cuda):
     for got, ref in zip(outs, want):
         for a, b in zip(got, ref):
             assert torch.equal(a.double(), b)
+
+
+def test_weights_quantised_on_a_stream_of_their_own(ffn, cuda):
+    """Transposed weights, which are copied first, on a side stream, while the
+    current stream is busy and takes new memory at once: the bits of a call alone."""
+    import torch
+    g = torch.Generator(device=cuda).manual_seed(12)
+    w = torch.randn(6, 1024, 520, device=cuda, generator=g).transpose(1, 2)
+    bias = torch.randn(6, 520, device=cuda, generator=g)
+    want = ffn.Int8Matrix.quantize(w.contiguous(), bias)
+    busy = torch.randn(4096, 4096, device=cuda, generator=g)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(4):
+        for _ in range(4):
+            busy = busy @ busy * 1e-3
+        got = ffn.Int8Matrix.quantize(w, bias, stream=side)
+        spoil = torch.full((6, 520, 1024), float("nan"), device=cuda)
+        side.synchronize()
+        assert torch.equal(got.w, want.w) and torch.equal(got.scale, want.scale) and got.bias is bias
+        del spoil
+    torch.cuda.synchronize()

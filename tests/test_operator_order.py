@@ -32,3 +32,42 @@ def test_tensor_memory_is_taken_behind_the_wait_for_the_previous_kernel(source):
             found += 1
             assert 0 <= body.find("pdl_enter()") < allocs[0], name
     assert found == 1
+
+
+def test_quantised_weights_are_copied_on_the_stream_of_the_call(ffn, monkeypatch):
+    """Weights that are not contiguous are copied first.  The copy, the kernel
+    that reads it and the copy's memory have to belong to one stream, the call's."""
+    import contextlib
+    now, seen = ["current"], []
+
+    @contextlib.contextmanager
+    def on(t, stream):
+        now.append(stream)
+        yield
+        now.pop()
+
+    class Weights:
+        shape = (2, 40, 64)
+
+        def dim(self):
+            return 3
+
+        def reshape(self, *shape):
+            seen.append(("copied", now[-1]))
+            return self
+
+        def as_strided(self, *layout):
+            return self
+
+    class Matrix(ffn.Int8Matrix):
+        def __init__(self, w, scale, bias=None):
+            pass
+
+    def kernel(x, stream=None):
+        seen.append(("read", now[-1] if stream is None else stream))
+        return x, None
+    monkeypatch.setattr(ffn, "_on", on)
+    monkeypatch.setattr(ffn, "_dev", lambda t, stream: 0 if stream is None else -1)
+    monkeypatch.setattr(ffn, "quantize_int8", kernel)
+    Matrix.quantize(Weights(), stream="side")
+    assert seen == [("copied", "side"), ("read", "side")]
