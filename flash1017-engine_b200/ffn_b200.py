@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import subprocess
+import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "_build", "libffn_b200.so")
@@ -66,7 +67,7 @@ K_NAMES = ["xprep", "router", "topk", "group", "gateup_nvfp4", "down_nvfp4", "ga
 
 
 def build() -> str:
-    subprocess.run(["make", "-s", "-C", HERE, "-j8"], check=True)
+    subprocess.run(["make", "-s", "-C", HERE, "-j8", f"PYTHON={sys.executable}"], check=True)
     return LIB_PATH
 
 
@@ -822,10 +823,15 @@ class MoeLayer:
 # stay lean: torch's accessors below cost 0.1 us each, current_stream() 2.
 # The plain cases go through a CPython module (csrc/torch_calls.cpp) that makes
 # the outputs and calls the library; what it does not take (None) and everything
-# where it was not built comes through here.
-CALLS_PATH = os.path.join(HERE, "_build", "ffn_b200_torch.so")
+# where it was not built, or does not load, comes through here.
 _dts = None
 _T = _dev_now = _raw_stream = _calls = None
+
+
+def _calls_path():
+    """The module built for this Python and this torch."""
+    import torch
+    return os.path.join(HERE, "_build", f"ffn_b200_torch.{sys.implementation.cache_tag}.torch-{torch.__version__}.so")
 
 
 def _setup():
@@ -834,11 +840,18 @@ def _setup():
     _dts = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
     _dev_now, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
     lib()
-    if os.path.exists(CALLS_PATH):
+    path = _calls_path()
+    if os.path.exists(path):
         import importlib.util
-        spec = importlib.util.spec_from_file_location("ffn_b200_torch", CALLS_PATH)
-        _calls = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(_calls)
+        spec = importlib.util.spec_from_file_location("ffn_b200_torch", path)
+        try:
+            calls = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(calls)
+            _calls = calls
+        except ImportError as e:
+            import warnings
+            warnings.warn(f"{path} does not load, the row operators' calls go through ctypes: {e}", RuntimeWarning,
+                          stacklevel=3)
     _T = torch
 
 
