@@ -489,7 +489,8 @@ int check_desc(const char *what, const ffn_b200_block_norm_desc *d) {
   if (d->rows > 0x7fffffffu) return fail(FFN_B200_EINVAL, w + ": too many rows");
   if (d->gate_kind != FFN_B200_GATE_NONE && d->gate_kind != FFN_B200_GATE_CHANNEL && d->gate_kind != FFN_B200_GATE_TOKEN)
     return fail(FFN_B200_EINVAL, w + ": unknown gate_kind");
-  if ((d->gate_kind != FFN_B200_GATE_NONE) != (d->gate != nullptr))
+  const bool no_gates = d->rows == 0 && d->gate_kind == FFN_B200_GATE_TOKEN;  // an empty array's address is null
+  if (!no_gates && (d->gate_kind != FFN_B200_GATE_NONE) != (d->gate != nullptr))
     return fail(FFN_B200_EINVAL, w + ": gate and gate_kind go together");
   if (!(d->eps >= 0.f)) return fail(FFN_B200_EINVAL, w + ": eps must not be negative");
   if (((uintptr_t)d->post_w | (uintptr_t)d->pre_w | (uintptr_t)d->gate) % 4)
@@ -563,7 +564,7 @@ int ffn_b200_block_norm_bwd(const ffn_b200_block_norm_desc *d, const void *y, si
                             void *stream) {
   using namespace ffn::bn;
   if (int rc = check_desc("block_norm_bwd", d)) return rc;
-  if ((dpost_w && !d->post_w) || (dgate && !d->gate))
+  if ((dpost_w && !d->post_w) || (dgate && d->gate_kind == FFN_B200_GATE_NONE))
     return fail(FFN_B200_EINVAL, "block_norm_bwd: a gradient of a parameter that is not there");
   if (((uintptr_t)dpost_w | (uintptr_t)dgate | (uintptr_t)dpre_w) % 4)
     return fail(FFN_B200_EINVAL, "block_norm_bwd: parameter gradients must be 4-byte aligned");
