@@ -628,7 +628,7 @@ int ffn_b200_moe_permute(size_t n_tok, size_t top_k, size_t row_bytes, const voi
                          void *stream) {
   using namespace ffn::route;
   if (int rc = check_pairs("moe_permute", n_tok, top_k, out_rows)) return rc;
-  if (n_tok == 0) return 0;
+  if (n_tok == 0 || out_rows == 0) return 0;
   if (!x || !pos || !out) return fail(FFN_B200_EINVAL, "moe_permute: null pointer");
   if ((x_scale == nullptr) != (out_scale == nullptr))
     return fail(FFN_B200_EINVAL, "moe_permute: x_scale and out_scale go together");
