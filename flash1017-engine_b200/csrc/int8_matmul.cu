@@ -40,10 +40,19 @@ struct QuantArgs {
   uint32_t cols, n_vec;
 };
 
-// The framework's gated activation (flash1017.rs:7539) of gate g and up u; the
-// fast division is within 2 steps, and gives the limit 0 where exp(-g) leaves f32.
+// The framework's gated activation (flash1017.rs:7539) of gate g and up u.  The fast
+// division is within 2 steps, but gives 0 for a divisor above 2^126 (g below -87.3).
+// What it drops there is below 1.1e-35, which no code shows unless the whole row is
+// that small; such a row takes `SMALL`: from -64 down 1 + exp(-g) rounds to exp(-g),
+// and the quotient is g exp(g).  (Taken for every value it cost 8192 x 2048 bf16 33
+// us, 27 like this.)
+constexpr float kSmallRow = 1e-28f;
+template <bool SMALL>
 __device__ __forceinline__ float swiglu10(float g, float u) {
-  return fminf(__fdividef(g, 1.0f + expf(-g)), 10.0f) * fminf(fmaxf(u, -10.0f), 10.0f);
+  float silu;
+  if (SMALL && g < -64.f) silu = g * expf(g);
+  else silu = __fdividef(g, 1.0f + expf(-g));
+  return fminf(silu, 10.0f) * fminf(fmaxf(u, -10.0f), 10.0f);
 }
 
 // Persistent, a row per CTA at a time; thread l holds the columns of pieces l, l +
@@ -54,7 +63,7 @@ constexpr int kQuantStages = 2;
 template <typename T, int VEC, int NV, int MT, bool SWIGLU, bool STAGED>
 __global__ void __launch_bounds__(MT) quant_kernel(const QuantArgs a) {
   constexpr int W = SWIGLU ? 2 : 1;  // gate and up
-  __shared__ uint32_t s_red[2][32];
+  __shared__ uint32_t s_red[2][32], s_small[32];
   extern __shared__ __align__(16) uint8_t s_dyn[];  // stages [kQuantStages][W][NV][threads] of 16 bytes
   pdl_enter();
   const uint32_t l = threadIdx.x, L = blockDim.x;
@@ -83,41 +92,56 @@ __global__ void __launch_bounds__(MT) quant_kernel(const QuantArgs a) {
       fetch(stage == 0 ? kQuantStages - 1 : stage - 1, row + (long long)(kQuantStages - 1) * gridDim.x);
       asm volatile("cp.async.wait_group %0;" ::"n"(kQuantStages - 1) : "memory");
     }
+    auto piece = [&](int w, int i) {
+      if constexpr (STAGED) return *reinterpret_cast<const Raw<T, VEC> *>(st + ((stage * W + w) * NV + i) * L);
+      else return load_raw<T, VEC>((const T *)a.x + (size_t)row * a.ld_x + (size_t)w * a.cols, l + i * L);
+    };
 #pragma unroll
     for (int w = 0; w < W; ++w)
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (l + i * L < a.n_vec) {
-          if constexpr (STAGED) r[w][i] = *reinterpret_cast<const Raw<T, VEC> *>(st + ((stage * W + w) * NV + i) * L);
-          else r[w][i] = load_raw<T, VEC>((const T *)a.x + (size_t)row * a.ld_x + (size_t)w * a.cols, l + i * L);
-        }
-    stage = stage == kQuantStages - 1 ? 0 : stage + 1;
+        if (l + i * L < a.n_vec) r[w][i] = piece(w, i);
     float f[SWIGLU ? NV : 1][VEC];
+    // the activations of piece i, and the largest magnitude's bits
+    auto gated = [&](auto small, const Raw<T, VEC> &gate, const Raw<T, VEC> &up, int i, uint32_t &m) {
+      float u[VEC];
+      unpack<T, VEC>(gate, f[i]);
+      unpack<T, VEC>(up, u);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        // the clamps would hide a gate or an up that is not finite
+        const bool fin = isfinite(f[i][j]) && isfinite(u[j]);
+        f[i][j] = swiglu10<decltype(small)::value>(f[i][j], u[j]);
+        m = max(m, fin ? __float_as_uint(f[i][j]) & 0x7fffffffu : 0x7f800000u);
+      }
+    };
+    auto cta_max = [&](uint32_t m, uint32_t *s) {
+      m = __reduce_max_sync(0xffffffffu, m);
+      if (nw > 1) {
+        if (lane == 0) s[warp] = m;
+        __syncthreads();
+        m = __reduce_max_sync(0xffffffffu, lane < nw ? s[lane] : 0u);
+      }
+      return m;
+    };
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (l + i * L >= a.n_vec) continue;
-      if (SWIGLU) {
-        float u[VEC];
-        unpack<T, VEC>(r[0][i], f[i]);
-        unpack<T, VEC>(r[W - 1][i], u);
+      if constexpr (SWIGLU) gated(std::false_type(), r[0][i], r[W - 1][i], i, m);
+      else m = max(m, abs_bits<T, VEC>(r[0][i]));
+    }
+    m = cta_max(m, s_red[par]);
+    if constexpr (SWIGLU) {
+      if (m < __float_as_uint(kSmallRow)) {  // the whole CTA: m is the row's
+        m = 0;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          // the clamps would hide a gate or an up that is not finite
-          const bool fin = isfinite(f[i][j]) && isfinite(u[j]);
-          f[i][j] = swiglu10(f[i][j], u[j]);
-          m = max(m, fin ? __float_as_uint(f[i][j]) & 0x7fffffffu : 0x7f800000u);
-        }
-      } else {
-        m = max(m, abs_bits<T, VEC>(r[0][i]));
+        for (int i = 0; i < NV; ++i)
+          if (l + i * L < a.n_vec) gated(std::true_type(), piece(0, i), piece(W - 1, i), i, m);
+        m = cta_max(m, s_small);
       }
     }
-    m = __reduce_max_sync(0xffffffffu, m);
-    if (nw > 1) {
-      if (lane == 0) s_red[par][warp] = m;
-      __syncthreads();
-      m = __reduce_max_sync(0xffffffffu, lane < nw ? s_red[par][lane] : 0u);
-    }
+    stage = stage == kQuantStages - 1 ? 0 : stage + 1;
     const Int8Row sc = SWIGLU ? Int8Row(__uint_as_float(m)) : Int8Row::of_bits<T>(m);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
