@@ -569,7 +569,6 @@ __global__ void __launch_bounds__(threads_of(MB), 1) gemm_kernel(const GemmArgs 
 // of loads in flight an SM.
 constexpr int kFewRows = 2;
 constexpr int kFewThreads = 512;
-constexpr size_t kFewSmem = 47 * 1024;  // the launch default, less the static part
 struct FewArgs {
   const void *x;
   size_t ld_x, ld_w, ld_out;
@@ -580,6 +579,8 @@ struct FewArgs {
   bool x16;  // x's rows can be read 16 bytes at a time
 };
 __host__ __device__ constexpr int few_pitch(int k) { return (k + 4095) / 4096 * 4096; }  // code bytes a token
+constexpr int kFewCols = 16384;
+static_assert(kFewRows * few_pitch(kFewCols) <= 47 * 1024, "the codes fit the launch default, less the static part");
 
 // 16 weights from column 16 p of a row (zeros past k)
 __device__ __forceinline__ uint4 few_piece(const int8_t *row, int p, int k) {
@@ -702,7 +703,7 @@ int launch_few(const FewArgs &a, int rows, int sms, cudaStream_t st) {
   return 0;
 }
 bool few_fits(size_t rows, size_t k, size_t n_groups, const int32_t *offsets) {
-  return rows <= (size_t)kFewRows && n_groups == 1 && !offsets && k <= 16384 && rows * few_pitch((int)k) <= kFewSmem;
+  return rows <= (size_t)kFewRows && n_groups == 1 && !offsets && k <= (size_t)kFewCols;
 }
 
 // ------------------------------------------------------------------ launch
