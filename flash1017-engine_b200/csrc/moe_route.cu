@@ -25,10 +25,11 @@ namespace route {
 // with the same expert, found by a ballot per bit of the expert number, in lane
 // order), so the order inside an expert is the pair order.  match.any finds the
 // same lanes in one instruction, but its latency was most of the kernel's time.
-// Counts per (segment, expert) sit in shared memory; the CTAs of the cluster read each other's totals over distributed
-// shared memory, which saves the second and third launch and the workspace
-// that a grid-wide sort would need.  Bound by latency, not by bytes: 8 bytes
-// a pair.
+// Counts per (segment, expert) sit in shared memory; the CTAs of the cluster read
+// each other's totals over distributed shared memory, which saves the second and
+// third launch and the workspace that a grid-wide sort would need.  Bound by
+// latency, not by bytes: 8 bytes a pair.  src is scattered by the same kernel
+// (49152 pairs: 9.5 us; 10.0 with a second kernel that wrote it from pos).
 constexpr int kSortThreads = 1024;
 constexpr int kSortCluster = 16;    // most CTAs of a cluster (8 are portable)
 constexpr int kSortBatch = 8;
@@ -74,7 +75,7 @@ __device__ __forceinline__ uint32_t same_lanes(uint32_t v, int bits) {
 }
 
 __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortArgs a) {
-  extern __shared__ int s_cnt[];  // [segs][n_local], then [n_local] totals, then [n_local + 1] offsets
+  extern __shared__ int s_cnt[];  // [segs][n_local], then [n_local] totals, then [n_local] first rows
   __shared__ int s_warp[32];
   __shared__ int s_carry;
   pdl_enter();
@@ -209,20 +210,6 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortArgs a)
       a.src[r] = -1;
   __syncwarp();
   cluster_wait();
-}
-
-// src from pos, for many pairs: their scattered 4-byte stores take one SM 32
-// cycles a warp, which the sort's 8 CTAs cannot hide (49152 pairs: 12.0 us with
-// src written by the sort, 11.0 us with this kernel behind it).
-constexpr int kSrcPairs = 16384;
-__global__ void __launch_bounds__(256) src_kernel(const int32_t *pos, const int32_t *total, int32_t *src, int n_pairs) {
-  pdl_enter();
-  const int n = *total;
-  for (int p = blockIdx.x * 256 + threadIdx.x; p < n_pairs; p += gridDim.x * 256) {
-    const uint32_t r = (uint32_t)pos[p];
-    if (r < (uint32_t)n_pairs) src[r] = p;
-    if (p >= n) src[p] = -1;
-  }
 }
 
 // Work layout of the row kernels: `tpt` threads (a power of two, 32 .. 256) share
@@ -563,11 +550,10 @@ int ffn_b200_moe_sort(size_t n_tok, size_t top_k, const int32_t *idx, int32_t ex
   a.n_local = expert_end - expert_begin;
   a.offsets = offsets;
   a.pos = pos;
-  const bool later = src && pos && a.n_pairs > kSrcPairs;
-  a.src = later ? nullptr : src;
+  a.src = src;
   // One CTA up to 512 pairs (384 experts: 4.5 us for 384 pairs, but 7.3 us for 2046
   // against 4.5 us with the cluster).
-  // Above 8192 pairs 16 CTAs (49152 pairs: 11.0 us with 8, 9.8 us), where this
+  // Above 8192 pairs 16 CTAs (49152 pairs: 12.0 us with 8, 9.5 us), where this
   // GPU can hold such a cluster.
   static int widest[64] = {0};
   if (!widest[dev]) {
@@ -617,9 +603,6 @@ int ffn_b200_moe_sort(size_t n_tok, size_t top_k, const int32_t *idx, int32_t ex
     (void)cudaGetLastError();
     return cuda_fail(e, "moe_sort");
   }
-  if (later)
-    FFN_LAUNCH_PDL(FFN_B200_K_ROUTE, st, "moe_sort src", src_kernel, grid_of((a.n_pairs + 255) / 256, 8), 256, 0, pos,
-                   offsets + a.n_local, src, a.n_pairs);
   return 0;
 }
 
