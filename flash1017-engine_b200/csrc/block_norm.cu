@@ -438,10 +438,13 @@ int launch_fwd(FwdArgs &a, cudaStream_t st) {
   return launch_fwd_as<T, VEC, 16 / VEC, 1024>(a, st);
 }
 
-// Backward: 8 columns a thread (about 90 registers) for f32 up to 5120 columns,
-// where the staged rows leave room for one CTA an SM anyway, for 16-bit types up
-// to 1024, and for single elements (more would spill); else 16, which halves the
-// reductions' share of the instructions.
+// Backward: 8 columns a thread (about 90 registers) up to 5120 columns for f32,
+// where the staged rows leave room for one CTA an SM anyway, and for single
+// elements, and up to 1024 for 16-bit types; else 16, which halves the reductions'
+// share of the instructions.  Above 8192 columns that is a CTA of up to 1024 threads
+// with 64 registers each, which spills (bf16 628 bytes stored and 672 loaded a
+// thread, single elements 1246 and 1128) and has no stages: 2048 x 16384 bf16 takes
+// 217 us, where its bytes would take 62.
 constexpr int kStageMax = 224 * 1024;
 struct BwdShape {
   int per, threads;  // columns a thread, threads

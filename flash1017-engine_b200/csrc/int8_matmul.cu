@@ -809,10 +809,11 @@ int plan_gemm(GemmPlan &p, size_t rows, size_t n, size_t k, size_t n_groups, con
   p.mb = 1;
   if (offsets) {
     // Groups: bound by the weights' bytes, so one chunk should hold a group: the
-    // average and three deviations of an even routing (48 experts, K 2048, 128 rows
-    // each: 85 us with 160 rows a tile, 93 with 256, 94 with 128).  Two blocks of
-    // channels only for full tiles of 256 rows (512 rows each: 373 us, 435 with
-    // one; 128 rows each: 92 with two).
+    // average and three deviations of an even routing.  Two blocks of channels only
+    // for full tiles of 256 rows.  48 experts, K 2048, 4096 channels, f32 out, the
+    // product alone: 128 rows each 92 us (tiles of 176 rows; 160 91, 128 97, 256 98;
+    // two blocks of channels 93), 512 rows each 223 us (one block 241).
+    // The average is over all rows given, also those behind the last group.
     const double avg = (double)rows / n_groups, want = avg + 3 * sqrt(avg);
     a.nt = want >= 256 ? 256 : std::max(16, ((int)ceil(want) + 15) / 16 * 16);
     if (want > 256 && n > (size_t)kM) p.mb = 2;

@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(256) permute_kernel(const uint8_t *x, size_t l
 // A thread's piece of AHEAD routed rows is loaded before the first is used.
 // DRAM-bound by the experts' rows, so what counts is loads on their way: with 6
 // ahead 64 registers are enough and 1024 threads an SM fit (8 ahead and 768
-// threads: 24576 rows of 4096 bf16 take 61 us, like this 52).
+// threads: 24576 rows of 4096 bf16 and a residual take 61 us, like this 52).
 // Single elements (VEC 1) go four to a thread, so that looking a row up is not
 // most of the instructions (8192 x 6 x 4095 bf16: 501 us with one, 165 us).
 template <typename T, int VEC, int AHEAD>
@@ -340,8 +340,8 @@ __global__ void __launch_bounds__(256, AHEAD > 6 ? 3 : 4) combine_rows_kernel(co
 // TPT threads (one warp, or the CTA) a token: the token's gradient row is read
 // once per kBack choices (again from L1), each choice's row of y once, each row
 // of dy written once; the kBack dot products are reduced together.  kBack = 8
-// took 150 registers, one CTA an SM (4096 tokens x 6 x 4096 bf16, with dx: 193
-// us; 4: 149 us).
+// takes 128 registers, two CTAs an SM (4096 tokens x 6 x 4096 bf16: 93 us; 4: 79
+// us).
 constexpr int kBack = 4;
 template <typename T, int VEC, int TPT>
 __global__ void __launch_bounds__(256, 3) combine_bwd_kernel(const T *dout, size_t ld_d, const T *y, size_t ld_y,

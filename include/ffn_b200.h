@@ -328,9 +328,10 @@ FFN_B200_EXPORT int ffn_b200_quantize_int8(size_t rows, size_t cols, int32_t dty
                                            int32_t act, const int32_t *n_rows, int8_t *codes, size_t ld_codes,
                                            float *scales, void *stream);
 /* out[r][j] = x_scales[r] * w_scales[g][j] * sum_i x[r][i] w[g][j][i] + bias[g][j],
- * the sum exact in int32 (k <= 131072), out in dtype.  x [rows][ld_x] codes, w
- * [n_groups][n][ld_w] codes (groups contiguous), w_scales and bias (or NULL)
- * [n_groups][n] f32.  offsets DEVICE [n_groups + 1]: group g has the rows
+ * the sum exact in int32 (k <= 131072, x's codes within +-127 as quantize_int8 makes
+ * them: -128 times -128 in all 131072 places would not fit), out in dtype.  x
+ * [rows][ld_x] codes, w [n_groups][n][ld_w] codes (groups contiguous), w_scales and
+ * bias (or NULL) [n_groups][n] f32.  offsets DEVICE [n_groups + 1]: group g has the rows
  * offsets[g] .. offsets[g + 1] - 1, as moe_sort writes them (ascending; values
  * outside 0..rows are clamped); NULL: one group of all rows.  Rows in no group
  * are left as they were.  x, w 16-byte aligned, ld_x and ld_w multiples of 16;
