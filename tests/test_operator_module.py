@@ -29,7 +29,6 @@ def test_a_module_that_does_not_load(fresh, tmp_path, monkeypatch):
     bad = tmp_path / "ffn_b200_torch.so"
     bad.write_bytes(b"not a shared object")
     monkeypatch.setattr(fresh, "_calls_path", lambda: str(bad), raising=False)
-    monkeypatch.setattr(fresh, "CALLS_PATH", str(bad), raising=False)
     with pytest.warns(RuntimeWarning, match="ctypes"):
         refuses_as_ever(fresh)
     assert fresh._calls is None and fresh._T is not None
